@@ -194,6 +194,105 @@ int ltc_preamble_backward(int64_t rows, int32_t D, const float* x, const float* 
                           float* g_ln_b, float* g_in_w, float* g_in_b, void* workspace, size_t workspace_bytes,
                           ltc_stream_t stream);
 
+/* ---- Sequence operators beside the solver (no counterpart in the reference) ---------
+ * Inputs and gradients of these calls are fp32, bf16 or fp16 (LTC_DTYPE_*); states,
+ * decay, sums and statistics are fp32. */
+enum { LTC_DTYPE_F32 = 0, LTC_DTYPE_BF16 = 1, LTC_DTYPE_F16 = 2 };
+
+/* Linear recurrences, parallel over time (ltc_forward walks its T * ode_unfolds unfolds one
+ * after the other).  Per channel, inside one sequence:
+ *   linear   h_t = a_t h_{t-1} + b_t
+ *   gated    L_t = -scale softplus(decay) sigmoid(rate_t),  a_t = exp(L_t),
+ *            h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(gate_t) x_t
+ * Padded batches: inputs (B,T,H), states (B,H), num_seqs = 0, seq_starts NULL.
+ * Packed sequences: B = 1, T = all tokens, num_seqs = S >= 1, states (S,H), and seq_starts
+ * (S+1) non-decreasing token offsets ON THE DEVICE: sequence n holds tokens seq_starts[n] ..
+ * seq_starts[n+1]-1 (none: its first state is its final state).  Tokens outside every
+ * sequence give h = 0 and zero gradients, whatever they hold.  Offsets out of order give
+ * wrong numbers but no access out of bounds. */
+typedef struct {
+  int32_t B, T, H;
+  int32_t dtype;    /* of the inputs, h and their gradients */
+  int32_t num_seqs; /* 0: padded batch */
+} LtcScanDims;
+
+/* One (B,T,H) input: element strides of batch and time, channels contiguous. */
+typedef struct {
+  const void* data;
+  int64_t stride_b, stride_t;
+} LtcScanInput;
+
+/* saved_bytes: state before each tile of `tile` tokens, kept by a forward for its backward
+ * (0 when one tile covers a row).  segments: parts that time is cut into when there are
+ * too few (sequence, channel) chains to fill the GPU. */
+typedef struct {
+  size_t saved_bytes, fwd_workspace_bytes, bwd_workspace_bytes;
+  int32_t tile, segments;
+} LtcScanPlan;
+
+int ltc_scan_plan(const LtcScanDims* dims, LtcScanPlan* out);
+
+/* h0 may be NULL (zeros) and must not be the h_final array.  saved may be NULL when no
+ * backward follows or plan.saved_bytes is 0.  h (B,T,H) is written contiguously.  Deterministic. */
+int ltc_linear_scan_forward(const LtcScanDims* dims, const LtcScanInput* a, const LtcScanInput* b, const float* h0,
+                            const int32_t* seq_starts, void* h, float* h_final, void* saved, void* workspace,
+                            size_t workspace_bytes, ltc_stream_t stream);
+int ltc_gated_scan_forward(const LtcScanDims* dims, const LtcScanInput* x, const LtcScanInput* rate,
+                           const LtcScanInput* gate, const float* decay, float scale, const float* h0,
+                           const int32_t* seq_starts, void* h, float* h_final, void* saved, void* workspace,
+                           size_t workspace_bytes, ltc_stream_t stream);
+/* Gradients, contiguous.  dh (NULL: none) is the gradient of h, dh_final (NULL: none) that
+ * of h_final; dh0 may be NULL.  The states are rebuilt from `saved`, h is not read. */
+int ltc_linear_scan_backward(const LtcScanDims* dims, const LtcScanInput* a, const LtcScanInput* b, const float* h0,
+                             const int32_t* seq_starts, const void* saved, const LtcScanInput* dh,
+                             const float* dh_final, void* da, void* db, float* dh0, void* workspace,
+                             size_t workspace_bytes, ltc_stream_t stream);
+int ltc_gated_scan_backward(const LtcScanDims* dims, const LtcScanInput* x, const LtcScanInput* rate,
+                            const LtcScanInput* gate, const float* decay, float scale, const float* h0,
+                            const int32_t* seq_starts, const void* saved, const LtcScanInput* dh,
+                            const float* dh_final, void* dx, void* drate, void* dgate, float* ddecay, float* dh0,
+                            void* workspace, size_t workspace_bytes, ltc_stream_t stream);
+/* One token for each of B sequences (dims.T and num_seqs are ignored, stride_t too): h (B,H)
+ * and state_out (B,H), which may be the state array itself.  state may be NULL (zeros). */
+int ltc_gated_scan_step(const LtcScanDims* dims, const LtcScanInput* x, const LtcScanInput* rate,
+                        const LtcScanInput* gate, const float* decay, float scale, const float* state, void* h,
+                        float* state_out, ltc_stream_t stream);
+
+/* Logits z (rows, V), V contiguous; row r starts at element (r / inner_rows) * stride_outer +
+ * (r % inner_rows) * stride_inner, so that a slice of a (B,T,V) tensor needs no copy.
+ * q = softmax(z / temperature).  A row of nothing but -inf has no distribution: its log
+ * probabilities are -inf, its entropy 0, its gradient 0.  NaN and +inf give NaN rows. */
+typedef struct {
+  const void* data;
+  int64_t rows, inner_rows, stride_outer, stride_inner;
+  int32_t V, dtype;
+  float temperature;
+} LtcLogits;
+
+/* Distillation from the K <= 256 best entries of a teacher: p = softmax(teacher / tau) over
+ * the entries of a row with id >= 0, loss[row] = tau^2 sum_k p_k (log p_k - log q_{id_k}).
+ * A row without entries costs 0 and has no gradient; an id given twice counts twice; an id
+ * >= V makes the row NaN.  teacher (rows, K) of teacher_dtype and ids are contiguous.  probs
+ * (rows, K) and stats (rows, 4; 16-byte aligned) are kept for the backward, or both NULL. */
+int ltc_distill_forward(const LtcLogits* logits, const int64_t* ids, const void* teacher, int32_t teacher_dtype,
+                        int32_t K, float* loss, float* probs, float* stats, ltc_stream_t stream);
+/* dlogits (rows, V) contiguous; g_loss is read with element stride g_stride (0 or 1). */
+int ltc_distill_backward(const LtcLogits* logits, const int64_t* ids, int32_t K, const float* probs,
+                         const float* stats, const float* g_loss, int64_t g_stride, void* dlogits,
+                         ltc_stream_t stream);
+
+/* Log probability of one given token a row (token < 0: none, 0 is written; >= V: NaN), the
+ * row's entropy, and its top_k <= 64 largest log probabilities, best first, ties to the
+ * lowest id; where fewer entries are above -inf, id -1 and -inf.  top_ids / top_logprobs
+ * (rows, top_k) are not read when top_k is 0.  stats as above, or NULL. */
+int ltc_token_logprobs_forward(const LtcLogits* logits, const int64_t* tokens, int32_t top_k, float* logprobs,
+                               float* entropy, int64_t* top_ids, float* top_logprobs, float* stats,
+                               ltc_stream_t stream);
+/* Gradient of log probabilities and entropies; each of the two may be NULL (none). */
+int ltc_token_logprobs_backward(const LtcLogits* logits, const int64_t* tokens, const float* stats,
+                                const float* g_logprob, int64_t g_logprob_stride, const float* g_entropy,
+                                int64_t g_entropy_stride, void* dlogits, ltc_stream_t stream);
+
 /* Size of the fixed device scratch array behind ltc_forward_noalloc (16 MiB per GPU). */
 #define LTC_NOALLOC_SCRATCH_BYTES (16u * 1024u * 1024u)
 
@@ -214,7 +313,8 @@ int ltc_forward_noalloc(const LtcDims* dims, const LtcParams* params, const floa
 
 /* Kernel identifiers of the launches each call issues (forward: PACK_FWD,
  * SENSORY_FWD, RECURRENT_FWD; backward: PACK_BWD, RECURRENT_BWD, SENSORY_BWD, FINISH; the fused
- * module preamble: PREAMBLE_FWD, PREAMBLE_BWD). */
+ * module preamble: PREAMBLE_FWD, PREAMBLE_BWD; the scans, the single-token step among the
+ * forward ones: SCAN_FWD, SCAN_BWD; the vocabulary operators: VOCAB_FWD, VOCAB_BWD). */
 enum {
   LTC_KERNEL_PACK_FWD = 0,
   LTC_KERNEL_SENSORY_FWD = 1,
@@ -225,15 +325,19 @@ enum {
   LTC_KERNEL_FINISH = 6,
   LTC_KERNEL_PREAMBLE_FWD = 7,
   LTC_KERNEL_PREAMBLE_BWD = 8,
-  LTC_NUM_KERNELS = 9
+  LTC_KERNEL_SCAN_FWD = 9,
+  LTC_KERNEL_SCAN_BWD = 10,
+  LTC_KERNEL_VOCAB_FWD = 11,
+  LTC_KERNEL_VOCAB_BWD = 12,
+  LTC_NUM_KERNELS = 13
 };
 
 /* Per-launch device timing, process-wide (no counterpart in the
  * reference, whose bench times with torch.profiler, bench_ltc.py:292-387).
  * While enabled, every launch is bracketed by a cudaEvent pair recorded on its
  * own stream.  ltc_timing_collect() waits for them, writes the summed
- * milliseconds and launch counts per LTC_KERNEL_* id (n >= LTC_NUM_KERNELS) and
- * clears the record. */
+ * milliseconds and launch counts per LTC_KERNEL_* id and clears the record.  n is the
+ * length of both arrays, at least 9; ids past it are left out. */
 int ltc_timing_enable(int on);
 int ltc_timing_collect(double* total_ms, int32_t* launches, int n);
 

@@ -298,7 +298,7 @@ int ltc_timing_enable(int on) {
 }
 
 int ltc_timing_collect(double* total_ms, int32_t* launches, int n) {
-  if (!total_ms || !launches || n < LTC_NUM_KERNELS) return fail("ltc_timing_collect: need %d slots", LTC_NUM_KERNELS);
+  if (!total_ms || !launches || n < 9) return fail("ltc_timing_collect: need at least 9 slots");
   std::lock_guard<std::mutex> lk(g_tm_mu);
   for (int k = 0; k < n; ++k) {
     total_ms[k] = 0.0;
@@ -310,6 +310,7 @@ int ltc_timing_collect(double* total_ms, int32_t* launches, int n) {
     float ms = 0.f;
     e = cudaEventElapsedTime(&ms, g_tm.start[i], g_tm.stop[i]);
     if (e != cudaSuccess) return cuda_fail(e, "cudaEventElapsedTime");
+    if (g_tm.kid[i] >= n) continue;
     total_ms[g_tm.kid[i]] += ms;
     launches[g_tm.kid[i]] += 1;
   }
@@ -877,6 +878,295 @@ int ltc_step_unfold_backward(const LtcDims* dims, const LtcParams* params, const
   if (e != cudaSuccess) return cuda_fail(e, "ltc_step_unfold_backward");
   g_last_error.clear();
   return 0;
+}
+
+// ---- sequence operators -----------------------------------------------------------
+
+namespace {
+
+struct ScanCall {
+  DeviceInfo di;
+  ScanPlan plan;
+  size_t agg_floats, part_floats, saved_floats;
+};
+
+int scan_begin(const LtcScanDims* d, const char* who, ScanCall* c) {
+  if (!d) return fail("%s: dims is NULL", who);
+  if (d->B < 1 || d->T < 1 || d->H < 1 || d->T > 0x7fffff00)
+    return fail("%s: need B, T, H >= 1 (got %d, %d, %d)", who, d->B, d->T, d->H);
+  if (d->dtype < 0 || d->dtype > LTC_DTYPE_F16) return fail("%s: unknown dtype %d", who, d->dtype);
+  if (d->num_seqs < 0 || (d->num_seqs > 0 && d->B != 1)) return fail("%s: packed sequences need B = 1", who);
+  int err = 0;
+  c->di = device_info(&err);
+  if (err) return 1;
+  c->plan = plan_scan(d->B, d->T, d->H, d->num_seqs > 0, c->di.sms);
+  const size_t bh = (size_t)d->B * d->H;
+  c->agg_floats = c->plan.nseg > 1 ? bh * c->plan.nseg * 2 : 0;
+  c->part_floats = bh * c->plan.nseg;
+  c->saved_floats = c->plan.tiles > 1 ? bh * c->plan.tiles : 0;
+  return 0;
+}
+
+size_t scan_carve(const ScanCall& c, bool bwd, void* ws, ScanArgs* a) {
+  Carver k(ws);
+  float* agg = c.agg_floats ? k.take<float>(c.agg_floats) : nullptr;
+  int* cut = c.agg_floats ? k.take<int>(c.plan.nseg) : nullptr;
+  float* part = bwd ? k.take<float>(c.part_floats) : nullptr;
+  if (a) {
+    a->agg = agg;
+    a->seg_cut = cut;
+    a->part = part;
+  }
+  return k.off ? k.off + 256 : 0;
+}
+
+// inputs and everything the two directions share
+int scan_args(const LtcScanDims* d, const ScanCall& c, const char* who, const LtcScanInput* const* in, int nin,
+              const float* h0, const int32_t* starts, bool bwd, void* ws, size_t ws_bytes, ScanArgs* a) {
+  for (int i = 0; i < nin; ++i) {
+    if (!in[i] || !in[i]->data) return fail("%s: input %d is NULL", who, i);
+    a->in[i] = in[i]->data;
+    a->sb[i] = in[i]->stride_b;
+    a->st[i] = in[i]->stride_t;
+  }
+  if ((d->num_seqs > 0) != (starts != nullptr)) return fail("%s: num_seqs and seq_starts go together", who);
+  const size_t need = scan_carve(c, bwd, nullptr, nullptr);
+  if (need > 0 && (!ws || ws_bytes < need))
+    return fail("%s: workspace of %zu bytes is smaller than the %zu bytes required", who, ws ? ws_bytes : 0, need);
+  scan_carve(c, bwd, need ? ws : nullptr, a);
+  a->h0 = h0;
+  a->starts = starts;
+  a->B = d->B; a->T = d->T; a->H = d->H; a->S = d->num_seqs;
+  a->tile = c.plan.tile; a->tiles = c.plan.tiles; a->seg_tiles = c.plan.seg_tiles; a->nseg = c.plan.nseg;
+  return 0;
+}
+
+int scan_forward(const LtcScanDims* d, const char* who, int policy, const LtcScanInput* const* in,
+                 const float* decay, float scale, const float* h0, const int32_t* starts, void* h, float* h_final,
+                 void* saved, void* ws, size_t ws_bytes, ltc_stream_t stream) {
+  ScanCall c;
+  if (scan_begin(d, who, &c)) return 1;
+  ScanArgs a{};
+  if (scan_args(d, c, who, in, policy ? 3 : 2, h0, starts, false, ws, ws_bytes, &a)) return 1;
+  if (!h || !h_final || (policy && !decay)) return fail("%s: NULL pointer", who);
+  if (h0 == h_final) return fail("%s: h_final must not be the h0 array", who);
+  a.decay = decay; a.scale = scale;
+  a.h = h; a.hT = h_final;
+  a.bounds = c.saved_floats ? static_cast<float*>(saved) : nullptr;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  {
+    TimedLaunch tl(LTC_KERNEL_SCAN_FWD, st);
+    e = launch_scan(a, policy, d->dtype, false, st);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  g_last_error.clear();
+  return 0;
+}
+
+int scan_backward(const LtcScanDims* d, const char* who, int policy, const LtcScanInput* const* in,
+                  const float* decay, float scale, const float* h0, const int32_t* starts, const void* saved,
+                  const LtcScanInput* dh, const float* dh_final, void* const* grads, float* ddecay, float* dh0,
+                  void* ws, size_t ws_bytes, ltc_stream_t stream) {
+  ScanCall c;
+  if (scan_begin(d, who, &c)) return 1;
+  ScanArgs a{};
+  const int nin = policy ? 3 : 2;
+  if (scan_args(d, c, who, in, nin, h0, starts, true, ws, ws_bytes, &a)) return 1;
+  if (c.saved_floats && !saved) return fail("%s: saved is NULL", who);
+  if (policy && (!decay || !ddecay)) return fail("%s: NULL pointer", who);
+  for (int i = 0; i < nin; ++i) {
+    if (!grads[i]) return fail("%s: NULL pointer", who);
+    a.d[i] = grads[i];
+  }
+  if (dh && dh->data) {
+    a.dh = dh->data;
+    a.sb[3] = dh->stride_b;
+    a.st[3] = dh->stride_t;
+  }
+  a.decay = decay; a.scale = scale;
+  a.bounds = const_cast<float*>(static_cast<const float*>(saved));
+  a.dhT = dh_final; a.dh0 = dh0; a.ddecay = ddecay;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  {
+    TimedLaunch tl(LTC_KERNEL_SCAN_BWD, st);
+    e = launch_scan(a, policy, d->dtype, true, st);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  g_last_error.clear();
+  return 0;
+}
+
+int vocab_args(const LtcLogits* z, const char* who, VocabArgs* a, DeviceInfo* di) {
+  if (!z || !z->data) return fail("%s: logits is NULL", who);
+  if (z->rows < 1 || z->inner_rows < 1 || z->V < 1 || z->V > (1 << 30))
+    return fail("%s: need rows, inner_rows >= 1 and 1 <= V <= 2^30", who);
+  if (z->dtype < 0 || z->dtype > LTC_DTYPE_F16) return fail("%s: unknown dtype %d", who, z->dtype);
+  if (!(z->temperature > 0.f) || !(z->temperature < 1e30f)) return fail("%s: temperature must be positive", who);
+  int err = 0;
+  *di = device_info(&err);
+  if (err) return 1;
+  a->z = z->data; a->rows = z->rows; a->n1 = z->inner_rows; a->s0 = z->stride_outer; a->s1 = z->stride_inner;
+  a->V = z->V; a->tau = z->temperature; a->inv_tau = 1.f / z->temperature;
+  return 0;
+}
+
+int vocab_launch(const VocabArgs& a, const LtcLogits* z, bool distill, bool bwd, int sms, const char* who,
+                 ltc_stream_t stream) {
+  if (reinterpret_cast<uintptr_t>(a.stats) % 16) return fail("%s: stats must be 16-byte aligned", who);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  {
+    TimedLaunch tl(bwd ? LTC_KERNEL_VOCAB_BWD : LTC_KERNEL_VOCAB_FWD, st);
+    e = bwd ? launch_vocab_bwd(a, z->dtype, distill, st) : launch_vocab_fwd(a, z->dtype, distill, sms, st);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  g_last_error.clear();
+  return 0;
+}
+
+}  // namespace
+
+int ltc_scan_plan(const LtcScanDims* dims, LtcScanPlan* out) {
+  if (!out) return fail("ltc_scan_plan: out is NULL");
+  ScanCall c;
+  if (scan_begin(dims, "ltc_scan_plan", &c)) return 1;
+  out->saved_bytes = c.saved_floats * sizeof(float);
+  out->fwd_workspace_bytes = scan_carve(c, false, nullptr, nullptr);
+  out->bwd_workspace_bytes = scan_carve(c, true, nullptr, nullptr);
+  out->tile = c.plan.tile;
+  out->segments = c.plan.nseg;
+  g_last_error.clear();
+  return 0;
+}
+
+int ltc_linear_scan_forward(const LtcScanDims* dims, const LtcScanInput* a, const LtcScanInput* b, const float* h0,
+                            const int32_t* seq_starts, void* h, float* h_final, void* saved, void* workspace,
+                            size_t workspace_bytes, ltc_stream_t stream) {
+  const LtcScanInput* in[] = {a, b};
+  return scan_forward(dims, "ltc_linear_scan_forward", 0, in, nullptr, 0.f, h0, seq_starts, h, h_final, saved,
+                      workspace, workspace_bytes, stream);
+}
+
+int ltc_gated_scan_forward(const LtcScanDims* dims, const LtcScanInput* x, const LtcScanInput* rate,
+                           const LtcScanInput* gate, const float* decay, float scale, const float* h0,
+                           const int32_t* seq_starts, void* h, float* h_final, void* saved, void* workspace,
+                           size_t workspace_bytes, ltc_stream_t stream) {
+  const LtcScanInput* in[] = {x, rate, gate};
+  return scan_forward(dims, "ltc_gated_scan_forward", 1, in, decay, scale, h0, seq_starts, h, h_final, saved,
+                      workspace, workspace_bytes, stream);
+}
+
+int ltc_linear_scan_backward(const LtcScanDims* dims, const LtcScanInput* a, const LtcScanInput* b, const float* h0,
+                             const int32_t* seq_starts, const void* saved, const LtcScanInput* dh,
+                             const float* dh_final, void* da, void* db, float* dh0, void* workspace,
+                             size_t workspace_bytes, ltc_stream_t stream) {
+  const LtcScanInput* in[] = {a, b};
+  void* grads[] = {da, db};
+  return scan_backward(dims, "ltc_linear_scan_backward", 0, in, nullptr, 0.f, h0, seq_starts, saved, dh, dh_final,
+                       grads, nullptr, dh0, workspace, workspace_bytes, stream);
+}
+
+int ltc_gated_scan_backward(const LtcScanDims* dims, const LtcScanInput* x, const LtcScanInput* rate,
+                            const LtcScanInput* gate, const float* decay, float scale, const float* h0,
+                            const int32_t* seq_starts, const void* saved, const LtcScanInput* dh,
+                            const float* dh_final, void* dx, void* drate, void* dgate, float* ddecay, float* dh0,
+                            void* workspace, size_t workspace_bytes, ltc_stream_t stream) {
+  const LtcScanInput* in[] = {x, rate, gate};
+  void* grads[] = {dx, drate, dgate};
+  return scan_backward(dims, "ltc_gated_scan_backward", 1, in, decay, scale, h0, seq_starts, saved, dh, dh_final,
+                       grads, ddecay, dh0, workspace, workspace_bytes, stream);
+}
+
+int ltc_gated_scan_step(const LtcScanDims* dims, const LtcScanInput* x, const LtcScanInput* rate,
+                        const LtcScanInput* gate, const float* decay, float scale, const float* state, void* h,
+                        float* state_out, ltc_stream_t stream) {
+  const char* who = "ltc_gated_scan_step";
+  if (!dims) return fail("%s: dims is NULL", who);
+  LtcScanDims d = *dims;
+  d.T = 1;
+  d.num_seqs = 0;
+  ScanCall c;
+  if (scan_begin(&d, who, &c)) return 1;
+  const LtcScanInput* in[] = {x, rate, gate};
+  ScanArgs a{};
+  if (scan_args(&d, c, who, in, 3, state, nullptr, false, nullptr, 0, &a)) return 1;
+  if (!h || !state_out || !decay) return fail("%s: NULL pointer", who);
+  for (int i = 0; i < 3; ++i) a.st[i] = 0;
+  a.decay = decay; a.scale = scale;
+  a.h = h; a.hT = state_out;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  {
+    TimedLaunch tl(LTC_KERNEL_SCAN_FWD, st);
+    e = launch_gated_step(a, d.dtype, st);
+  }
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  g_last_error.clear();
+  return 0;
+}
+
+int ltc_distill_forward(const LtcLogits* logits, const int64_t* ids, const void* teacher, int32_t teacher_dtype,
+                        int32_t K, float* loss, float* probs, float* stats, ltc_stream_t stream) {
+  const char* who = "ltc_distill_forward";
+  VocabArgs a{};
+  DeviceInfo di;
+  if (vocab_args(logits, who, &a, &di)) return 1;
+  if (K < 1 || K > kVocabMaxTeacher) return fail("%s: need 1 <= K <= %d", who, kVocabMaxTeacher);
+  if (teacher_dtype < 0 || teacher_dtype > LTC_DTYPE_F16) return fail("%s: unknown dtype %d", who, teacher_dtype);
+  if (!ids || !teacher || !loss || !probs != !stats) return fail("%s: NULL pointer", who);
+  a.ids = reinterpret_cast<const long long*>(ids);
+  a.teacher = teacher; a.teacher_dtype = teacher_dtype; a.K = K;
+  a.loss = loss; a.probs = probs; a.stats = stats;
+  return vocab_launch(a, logits, true, false, di.sms, who, stream);
+}
+
+int ltc_distill_backward(const LtcLogits* logits, const int64_t* ids, int32_t K, const float* probs,
+                         const float* stats, const float* g_loss, int64_t g_stride, void* dlogits,
+                         ltc_stream_t stream) {
+  const char* who = "ltc_distill_backward";
+  VocabArgs a{};
+  DeviceInfo di;
+  if (vocab_args(logits, who, &a, &di)) return 1;
+  if (K < 1 || K > kVocabMaxTeacher) return fail("%s: need 1 <= K <= %d", who, kVocabMaxTeacher);
+  if (!ids || !probs || !stats || !g_loss || !dlogits) return fail("%s: NULL pointer", who);
+  a.ids = reinterpret_cast<const long long*>(ids);
+  a.K = K; a.probs = const_cast<float*>(probs); a.stats = const_cast<float*>(stats);
+  a.g0 = g_loss; a.g0_stride = g_stride; a.dz = dlogits;
+  return vocab_launch(a, logits, true, true, di.sms, who, stream);
+}
+
+int ltc_token_logprobs_forward(const LtcLogits* logits, const int64_t* tokens, int32_t top_k, float* logprobs,
+                               float* entropy, int64_t* top_ids, float* top_logprobs, float* stats,
+                               ltc_stream_t stream) {
+  const char* who = "ltc_token_logprobs_forward";
+  VocabArgs a{};
+  DeviceInfo di;
+  if (vocab_args(logits, who, &a, &di)) return 1;
+  if (top_k < 0 || top_k > kVocabMaxTop || top_k > logits->V)
+    return fail("%s: need 0 <= top_k <= min(%d, V)", who, kVocabMaxTop);
+  if (!tokens || !logprobs || !entropy || (top_k > 0 && (!top_ids || !top_logprobs)))
+    return fail("%s: NULL pointer", who);
+  a.tokens = reinterpret_cast<const long long*>(tokens);
+  a.k = top_k; a.logprob = logprobs; a.entropy = entropy;
+  a.top_ids = reinterpret_cast<long long*>(top_ids); a.top_logprob = top_logprobs; a.stats = stats;
+  return vocab_launch(a, logits, false, false, di.sms, who, stream);
+}
+
+int ltc_token_logprobs_backward(const LtcLogits* logits, const int64_t* tokens, const float* stats,
+                                const float* g_logprob, int64_t g_logprob_stride, const float* g_entropy,
+                                int64_t g_entropy_stride, void* dlogits, ltc_stream_t stream) {
+  const char* who = "ltc_token_logprobs_backward";
+  VocabArgs a{};
+  DeviceInfo di;
+  if (vocab_args(logits, who, &a, &di)) return 1;
+  if (!tokens || !stats || !dlogits) return fail("%s: NULL pointer", who);
+  a.tokens = reinterpret_cast<const long long*>(tokens);
+  a.stats = const_cast<float*>(stats);
+  a.g0 = g_logprob; a.g0_stride = g_logprob_stride; a.g1 = g_entropy; a.g1_stride = g_entropy_stride;
+  a.dz = dlogits;
+  return vocab_launch(a, logits, false, true, di.sms, who, stream);
 }
 
 }  // extern "C"

@@ -206,6 +206,75 @@ int preamble_blocks(long long rows, int num_sms);
 cudaError_t launch_preamble_fwd(const PreambleArgs& a, int num_sms, cudaStream_t st);
 cudaError_t launch_preamble_bwd(const PreambleArgs& a, int num_sms, cudaStream_t st);
 
+// ---- linear recurrences over time (ltc_scan.cu) -----------------------------
+constexpr int kScanShortTile = 16, kScanLongTile = 64;  // tokens per tile
+struct ScanArgs {
+  const void* in[3];        // linear: a, b; gated: x, rate, gate
+  const void* dh;           // gradient of h (backward) or null
+  long long sb[4], st[4];   // batch and time strides (elements) of in[0..2] and dh; channels are contiguous
+  const float* decay;       // (H), gated
+  const float* h0;          // (B or S, H) or null (zeros)
+  const float* dhT;         // gradient of the final state, (B or S, H) or null
+  const int* starts;        // (S+1) token offsets of packed sequences (B = 1) or null
+  void* h;                  // (B,T,H)
+  float* hT;                // (B or S, H)
+  float* bounds;            // (B, tiles, H) state before each tile; null when no backward follows
+  void* d[3];               // gradients of in[]
+  float* dh0;               // (B or S, H) or null
+  float* ddecay;            // (H), gated
+  float* agg;               // (B, nseg, 2, H) folds of the segments (nseg > 1)
+  int* seg_cut;             // (nseg) packed: whether the segment holds a sequence start
+  float* part;              // (B, nseg, H) partial decay gradients
+  int B, T, H, S;
+  float scale;
+  int tile, tiles, seg_tiles, nseg;  // ScanPlan
+  // set per launch
+  int chb, launch_segs;
+  long long items;
+  bool fold_only;
+};
+struct ScanPlan {
+  int tile;       // tokens per tile
+  int tiles;      // tiles of a row
+  int seg_tiles;  // tiles of a segment
+  int nseg;       // segments of a row
+};
+ScanPlan plan_scan(int B, int T, int H, bool packed, int num_sms);
+// policy 0: linear, 1: gated; dtype 0: fp32, 1: bf16, 2: fp16
+cudaError_t launch_scan(const ScanArgs& a, int policy, int dtype, bool bwd, cudaStream_t st);
+cudaError_t launch_gated_step(const ScanArgs& a, int dtype, cudaStream_t st);
+
+// ---- softmax over a vocabulary (ltc_vocab.cu) ---------------------------------
+constexpr int kVocabMaxTop = 64, kVocabMaxTeacher = 256;
+struct VocabArgs {
+  const void* z;             // logits; row r starts at (r / n1) * s0 + (r % n1) * s1
+  long long rows, n1, s0, s1;
+  int V;
+  float tau, inv_tau;
+  // distillation
+  const long long* ids;      // (rows, K), < 0: no entry
+  const void* teacher;       // (rows, K)
+  int teacher_dtype, K;
+  float* loss;               // (rows)
+  float* probs;              // (rows, K) teacher probabilities (backward)
+  // token scores
+  const long long* tokens;   // (rows), < 0: none
+  float* logprob;            // (rows)
+  float* entropy;            // (rows)
+  int k;
+  long long* top_ids;        // (rows, k)
+  float* top_logprob;        // (rows, k)
+  float* stats;              // (rows, 4): maximum, log2 of the sum, entropy or whether the row counts
+  // backward
+  const float* g0; const float* g1;  // gradients of loss or log probability, and of the entropy; or null
+  long long g0_stride, g1_stride;    // 0 or 1
+  void* dz;                  // (rows, V)
+  // set per launch
+  int cluster, chunk, chunks;
+};
+cudaError_t launch_vocab_fwd(VocabArgs a, int dtype, bool distill, int num_sms, cudaStream_t st);
+cudaError_t launch_vocab_bwd(VocabArgs a, int dtype, bool distill, cudaStream_t st);
+
 // Error reporting shared by every extern "C" entry point (ltc_last_error()).
 void set_last_error(const char* msg);
 

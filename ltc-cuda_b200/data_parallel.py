@@ -10,10 +10,12 @@ needs and nothing more (the forward pass communicates nothing).
 """
 from __future__ import annotations
 
-from typing import Iterable, List, Tuple
+from typing import Iterable, List, Optional, Tuple
 
 import torch
 import torch.distributed as dist
+
+import ltc_cuda
 
 
 def shard_range(total: int, rank: int, world: int) -> Tuple[int, int]:
@@ -58,12 +60,35 @@ class FlatGradBucket:
         return self.flat.numel() * self.flat.element_size()
 
 
-def training_step(model, x: torch.Tensor, bucket: FlatGradBucket, optimizer, group=None) -> torch.Tensor:
-    """Forward, sum loss, backward, gradient all-reduce (SUM), optimizer step."""
+def training_step(model, x: torch.Tensor, bucket: FlatGradBucket, optimizer, group=None,
+                  teacher: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                  temperature: float = 1.0) -> torch.Tensor:
+    """Forward, loss, backward, gradient all-reduce (SUM), optimizer step.
+
+    The loss is the sum of the outputs, or, with ``teacher = (ids, logits)`` of shape
+    ``(B, T, K)`` for this rank's shard, the sum of ``ltc_cuda.ltc_distill_loss`` over the
+    outputs taken as logits -- a sum either way, so the shards' gradients add up to the
+    whole batch's."""
     bucket.zero()
     out, _ = model(x)
-    loss = out.sum()
+    loss = out.sum() if teacher is None else ltc_cuda.ltc_distill_loss(out, *teacher, temperature=temperature).sum()
     loss.backward()
     bucket.all_reduce(group)
     optimizer.step()
     return loss.detach()
+
+
+@torch.no_grad()
+def evaluation_step(model, x: torch.Tensor, tokens: torch.Tensor, group=None,
+                    temperature: float = 1.0) -> torch.Tensor:
+    """fp64 ``(sum of log probabilities, sum of entropies, count)`` over the given tokens
+    (``(B, T)``, negative: padding) of all ranks' shards, the model's outputs taken as
+    logits (``ltc_cuda.ltc_token_logprobs``)."""
+    out, _ = model(x)
+    scores = ltc_cuda.ltc_token_logprobs(out, tokens, temperature=temperature)
+    given = tokens >= 0
+    sums = torch.stack([scores.logprobs.double().sum(),
+                        torch.where(given, scores.entropy, 0.0).double().sum(), given.double().sum()])
+    if dist.is_available() and dist.is_initialized() and dist.get_world_size(group) > 1:
+        dist.all_reduce(sums, op=dist.ReduceOp.SUM, group=group)
+    return sums

@@ -20,6 +20,11 @@ opaque buffer (per-unfold states and reciprocal denominators) instead of the
 (T,U,B,H) state stack plus the two sensory stacks, and every kernel runs on
 PyTorch's current stream instead of the legacy default stream.
 
+Beside the solver it offers operators of sequence models that the reference lacks:
+:func:`ltc_linear_scan`, :func:`ltc_gated_scan` and :func:`ltc_gated_scan_step` (linear
+recurrences, parallel over time), :func:`ltc_distill_loss` and :func:`ltc_token_logprobs`
+(losses and scores over a vocabulary).
+
 There is no fallback inside this module: on a machine with CUDA, a missing or
 unloadable library raises at import; calling ``ltc_cuda_forward`` without CUDA
 kernels raises ``RuntimeError``.
@@ -30,9 +35,10 @@ import ctypes
 import logging
 import os
 import threading
-from typing import List, Optional, Sequence
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 logger = logging.getLogger(__name__)
 
@@ -70,6 +76,29 @@ class LtcPlan(ctypes.Structure):
                 ("lean_chunk_steps", ctypes.c_int32)]
 
 
+class LtcScanDims(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "T", "H", "dtype", "num_seqs")]
+
+
+class LtcScanInput(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_b", ctypes.c_int64), ("stride_t", ctypes.c_int64)]
+
+
+class LtcScanPlan(ctypes.Structure):
+    _fields_ = [("saved_bytes", ctypes.c_size_t), ("fwd_workspace_bytes", ctypes.c_size_t),
+                ("bwd_workspace_bytes", ctypes.c_size_t), ("tile", ctypes.c_int32), ("segments", ctypes.c_int32)]
+
+
+class LtcLogits(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("rows", ctypes.c_int64), ("inner_rows", ctypes.c_int64),
+                ("stride_outer", ctypes.c_int64), ("stride_inner", ctypes.c_int64), ("V", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("temperature", ctypes.c_float)]
+
+
+_IN = ctypes.POINTER(LtcScanInput)
+_LOGITS = ctypes.POINTER(LtcLogits)
+_P, _I32, _I64, _F32, _SIZE = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+
 # Exported symbols and their C signatures (include/ltc_sm100.h).
 EXPORTS = {
     "ltc_plan": (ctypes.c_int, [ctypes.POINTER(LtcDims), ctypes.POINTER(LtcPlan)]),
@@ -101,6 +130,19 @@ EXPORTS = {
                                           ctypes.c_int]),
     "ltc_launch_count": (ctypes.c_int64, []),
     "ltc_wait_timeouts": (ctypes.c_int, []),
+    "ltc_scan_plan": (ctypes.c_int, [ctypes.POINTER(LtcScanDims), ctypes.POINTER(LtcScanPlan)]),
+    "ltc_linear_scan_forward": (ctypes.c_int, [ctypes.POINTER(LtcScanDims), _IN, _IN] + [_P] * 6 + [_SIZE, _P]),
+    "ltc_gated_scan_forward": (ctypes.c_int, [ctypes.POINTER(LtcScanDims), _IN, _IN, _IN, _P, _F32] + [_P] * 6
+                               + [_SIZE, _P]),
+    "ltc_linear_scan_backward": (ctypes.c_int, [ctypes.POINTER(LtcScanDims), _IN, _IN, _P, _P, _P, _IN] + [_P] * 5
+                                 + [_SIZE, _P]),
+    "ltc_gated_scan_backward": (ctypes.c_int, [ctypes.POINTER(LtcScanDims), _IN, _IN, _IN, _P, _F32, _P, _P, _P, _IN]
+                                + [_P] * 7 + [_SIZE, _P]),
+    "ltc_gated_scan_step": (ctypes.c_int, [ctypes.POINTER(LtcScanDims), _IN, _IN, _IN, _P, _F32] + [_P] * 4),
+    "ltc_distill_forward": (ctypes.c_int, [_LOGITS, _P, _P, _I32, _I32] + [_P] * 4),
+    "ltc_distill_backward": (ctypes.c_int, [_LOGITS, _P, _I32, _P, _P, _P, _I64, _P, _P]),
+    "ltc_token_logprobs_forward": (ctypes.c_int, [_LOGITS, _P, _I32] + [_P] * 6),
+    "ltc_token_logprobs_backward": (ctypes.c_int, [_LOGITS, _P, _P, _P, _I64, _P, _I64, _P, _P]),
     "ltc_last_error": (ctypes.c_char_p, []),
     "ltc_version": (ctypes.c_int, []),
 }
@@ -287,7 +329,7 @@ def _call_flags_now() -> int:
 
 
 KERNEL_NAMES = ("pack_fwd", "sensory_fwd", "recurrent_fwd", "pack_bwd", "recurrent_bwd", "sensory_bwd",
-                "finish", "preamble_fwd", "preamble_bwd")
+                "finish", "preamble_fwd", "preamble_bwd", "scan_fwd", "scan_bwd", "vocab_fwd", "vocab_bwd")
 
 
 def timing_enable(on: bool) -> None:
@@ -632,3 +674,408 @@ class LtcPreamble(torch.autograd.Function):
 def ltc_preamble(x, ln_w, ln_b, in_w, in_b, eps: float):
     """Fused LayerNorm + affine map over the last dimension (D <= 1024)."""
     return LtcPreamble.apply(x, ln_w, ln_b, in_w, in_b, eps)
+
+
+# ---------------------------------------------------------------------------
+# Linear recurrences, parallel over time
+# ---------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _typed(t, name: str, dtype=None, device=None) -> torch.Tensor:
+    """A tensor of one of the three operand types (``dtype`` and ``device`` where they are set already)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16 (got {t.dtype})")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
+    return t
+
+
+def _on_cuda(t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name} is on {t.device}: the sm_100a kernels need CUDA tensors (there is no CPU fallback)")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """Channels contiguous, any strides before them."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _scan_input(t: torch.Tensor) -> LtcScanInput:
+    """(B,T,H), (T,H) packed or (B,H) single tokens."""
+    if t.dim() == 3:
+        return LtcScanInput(t.data_ptr(), t.stride(0), t.stride(1))
+    return LtcScanInput(t.data_ptr(), t.stride(0), t.stride(0))
+
+
+def _current_stream(dev) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _scan_operands(names, tensors, h0, seq_starts):
+    """Checked operands of a scan: (inputs, h0, seq_starts, dims as (B, T, H, S))."""
+    first = _typed(tensors[0], names[0])
+    want = 3 if seq_starts is None else 2
+    if first.dim() != want:
+        raise ValueError(f"{names[0]} must be {'(B, T, H)' if want == 3 else '(tokens, H) with seq_starts'}, "
+                         f"got shape {tuple(first.shape)}")
+    for t, n in zip(tensors[1:], names[1:]):
+        _typed(t, n, first.dtype, first.device)
+        if t.shape != first.shape:
+            raise ValueError(f"{n} has shape {tuple(t.shape)}, expected {tuple(first.shape)}")
+    H = first.shape[-1]
+    if seq_starts is None:
+        B, T, S = first.shape[0], first.shape[1], 0
+    else:
+        if not isinstance(seq_starts, torch.Tensor) or seq_starts.dtype not in (torch.int32, torch.int64):
+            raise TypeError("seq_starts must be an int32 or int64 tensor")
+        if seq_starts.dim() != 1 or seq_starts.numel() < 2:
+            raise ValueError("seq_starts must hold S + 1 >= 2 token offsets")
+        if seq_starts.device != first.device:
+            raise ValueError(f"seq_starts is on {seq_starts.device}, expected {first.device}")
+        B, T, S = 1, first.shape[0], seq_starts.numel() - 1
+        seq_starts = seq_starts.to(torch.int32).contiguous()
+    if T > 0x7fffff00:
+        raise ValueError(f"{T} time steps are more than a row may have (2^31 - 256)")
+    if h0 is not None:
+        h0 = _as_f32(h0, first.device, "h0")
+        if tuple(h0.shape) != (S or B, H):
+            raise ValueError(f"h0 has shape {tuple(h0.shape)}, expected {(S or B, H)}")
+    _on_cuda(first, names[0])
+    return [_rows(t) for t in tensors], h0, seq_starts, (B, T, H, S)
+
+
+def _check_decay(decay, device, H: int, scale: float) -> torch.Tensor:
+    decay = _as_f32(decay, device, "decay")
+    if tuple(decay.shape) != (H,):
+        raise ValueError(f"decay has shape {tuple(decay.shape)}, expected {(H,)}")
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite (got {scale})")
+    return decay
+
+
+class _ScanFunction(torch.autograd.Function):
+    """Both scans: ``inputs`` are (a, b), or (x, rate, gate) with ``decay``."""
+
+    @staticmethod
+    def forward(ctx, decay, h0, seq_starts, dims, scale, needs_grad, *inputs):
+        lib = _require_kernels()
+        B, T, H, S = dims
+        first = inputs[0]
+        dev = first.device
+        ctx.dims, ctx.scale = dims, scale
+        ctx.set_materialize_grads(False)
+        h = torch.empty(first.shape, device=dev, dtype=first.dtype)
+        h_final = torch.empty(S or B, H, device=dev, dtype=torch.float32)
+        saved = None
+        if first.numel() == 0:
+            h_final.zero_() if h0 is None else h_final.copy_(h0)
+        else:
+            cd = LtcScanDims(B, T, H, _DTYPES[first.dtype], S)
+            ins = [ctypes.byref(_scan_input(t)) for t in inputs]
+            with torch.cuda.device(dev):
+                p = LtcScanPlan()
+                _check(lib.ltc_scan_plan(ctypes.byref(cd), ctypes.byref(p)), "ltc_scan_plan")
+                if needs_grad and p.saved_bytes:
+                    saved = torch.empty(p.saved_bytes, device=dev, dtype=torch.uint8)
+                ws = torch.empty(p.fwd_workspace_bytes, device=dev, dtype=torch.uint8)
+                tail = (_ptr(h0), _ptr(seq_starts), h.data_ptr(), h_final.data_ptr(), _ptr(saved), _ptr(ws),
+                        p.fwd_workspace_bytes, _current_stream(dev))
+                if decay is None:
+                    _check(lib.ltc_linear_scan_forward(ctypes.byref(cd), *ins, *tail), "ltc_linear_scan")
+                else:
+                    _check(lib.ltc_gated_scan_forward(ctypes.byref(cd), *ins, decay.data_ptr(), scale, *tail),
+                           "ltc_gated_scan")
+        if needs_grad:
+            ctx.save_for_backward(decay, h0, seq_starts, saved, *inputs)
+        return h, h_final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, dh_final):
+        lib = _require_kernels()
+        decay, h0, seq_starts, saved, *inputs = ctx.saved_tensors
+        B, T, H, S = ctx.dims
+        first = inputs[0]
+        dev = first.device
+        grads = [torch.empty(t.shape, device=dev, dtype=t.dtype) for t in inputs]
+        dh0 = None if h0 is None else torch.empty_like(h0)
+        ddecay = None if decay is None else torch.empty_like(decay)
+        if first.numel() == 0:
+            if dh0 is not None:
+                dh0.zero_() if dh_final is None else dh0.copy_(dh_final)
+            if ddecay is not None:
+                ddecay.zero_()
+            return (ddecay, dh0, None, None, None, None, *grads)
+        if dh is not None:
+            dh = _rows(dh.to(first.dtype))
+        if dh_final is not None:
+            dh_final = dh_final.to(torch.float32).contiguous()
+        cd = LtcScanDims(B, T, H, _DTYPES[first.dtype], S)
+        ins = [ctypes.byref(_scan_input(t)) for t in inputs]
+        with torch.cuda.device(dev):
+            p = LtcScanPlan()
+            _check(lib.ltc_scan_plan(ctypes.byref(cd), ctypes.byref(p)), "ltc_scan_plan")
+            ws = torch.empty(p.bwd_workspace_bytes, device=dev, dtype=torch.uint8)
+            mid = (_ptr(h0), _ptr(seq_starts), _ptr(saved), None if dh is None else ctypes.byref(_scan_input(dh)),
+                   _ptr(dh_final), *[g.data_ptr() for g in grads])
+            tail = (_ptr(dh0), ws.data_ptr(), p.bwd_workspace_bytes, _current_stream(dev))
+            if decay is None:
+                _check(lib.ltc_linear_scan_backward(ctypes.byref(cd), *ins, *mid, *tail), "ltc_linear_scan backward")
+            else:
+                _check(lib.ltc_gated_scan_backward(ctypes.byref(cd), *ins, decay.data_ptr(), ctx.scale, *mid,
+                                                   ddecay.data_ptr(), *tail), "ltc_gated_scan backward")
+        return (ddecay, dh0, None, None, None, None, *grads)
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def ltc_linear_scan(a, b, h0=None, seq_starts=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``h_t = a_t * h_{t-1} + b_t`` for every channel -> ``(h, h_final)``.
+
+    ``a``, ``b``: ``(B, T, H)``, or ``(tokens, H)`` packed sequences with ``seq_starts``
+    (``S + 1`` non-decreasing token offsets on the device, int32 or int64); fp32, bf16 or fp16, both the
+    same, any batch and time strides.  ``h0`` (fp32 ``(B, H)`` or ``(S, H)``) defaults to
+    zeros.  ``h`` has the type of the inputs, ``h_final`` is fp32, and so is the state in
+    between.  Tokens that belong to no sequence give 0 and get no gradient; a sequence
+    without tokens returns its ``h0``.  Differentiable once in ``a``, ``b`` and ``h0``."""
+    tensors, h0, seq_starts, dims = _scan_operands(("a", "b"), (a, b), h0, seq_starts)
+    return _ScanFunction.apply(None, h0, seq_starts, dims, 0.0, _wants_grad(*tensors, h0), *tensors)
+
+
+def ltc_gated_scan(x, rate, gate, decay, h0=None, seq_starts=None, scale: float = 8.0):
+    """Gated linear recurrence -> ``(h, h_final)``:
+
+    ``a_t = exp(-scale * softplus(decay) * sigmoid(rate_t))``,
+    ``h_t = a_t * h_{t-1} + sqrt(1 - a_t**2) * sigmoid(gate_t) * x_t``.
+
+    ``x``, ``rate``, ``gate`` like the inputs of :func:`ltc_linear_scan` (slices of one
+    projection need no copy), ``decay`` fp32 ``(H,)``; the gates are computed in fp32
+    inside the scan.  Differentiable once in all of them and ``h0``."""
+    tensors, h0, seq_starts, dims = _scan_operands(("x", "rate", "gate"), (x, rate, gate), h0, seq_starts)
+    decay = _check_decay(decay, tensors[0].device, dims[2], scale)
+    return _ScanFunction.apply(decay, h0, seq_starts, dims, float(scale), _wants_grad(*tensors, decay, h0), *tensors)
+
+
+def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_state=None):
+    """One token for each sequence: ``x``, ``rate``, ``gate`` ``(B, H)``, ``state`` fp32
+    ``(B, H)`` -> ``(h, new_state)``, what :func:`ltc_gated_scan` gives for ``T = 1``.
+    ``out_state`` receives the new state; ``out_state=state`` updates it in place.  Not
+    differentiable: raises where a gradient would be recorded."""
+    first = _typed(x, "x")
+    if first.dim() != 2:
+        raise ValueError(f"x must be (B, H), got shape {tuple(first.shape)}")
+    dev, (B, H) = first.device, first.shape
+    for t, n in ((rate, "rate"), (gate, "gate")):
+        _typed(t, n, first.dtype, dev)
+        if t.shape != first.shape:
+            raise ValueError(f"{n} has shape {tuple(t.shape)}, expected {tuple(first.shape)}")
+    _on_cuda(first, "x")
+    decay = _check_decay(decay, dev, H, scale)
+    s = _as_f32(state, dev, "state")
+    if s.shape != first.shape:
+        raise ValueError(f"state has shape {tuple(s.shape)}, expected {tuple(first.shape)}")
+    if _wants_grad(x, rate, gate, decay, state):
+        raise RuntimeError("ltc_gated_scan_step has no backward pass; use ltc_gated_scan or torch.no_grad()")
+    if out_state is None:
+        out_state = torch.empty(B, H, device=dev, dtype=torch.float32)
+    elif (not isinstance(out_state, torch.Tensor) or out_state.dtype != torch.float32 or out_state.device != dev
+          or out_state.shape != first.shape or not out_state.is_contiguous()):
+        raise ValueError("out_state must be a contiguous fp32 tensor shaped and placed like x")
+    elif 0 < abs(out_state.data_ptr() - s.data_ptr()) < 4 * s.numel():
+        raise ValueError("out_state may be state itself but not overlap it otherwise")
+    lib = _require_kernels()
+    h = torch.empty(B, H, device=dev, dtype=first.dtype)
+    if h.numel():
+        cd = LtcScanDims(B, 1, H, _DTYPES[first.dtype], 0)
+        ins = [ctypes.byref(_scan_input(_rows(t))) for t in (x, rate, gate)]
+        with torch.cuda.device(dev):
+            _check(lib.ltc_gated_scan_step(ctypes.byref(cd), *ins, decay.data_ptr(), float(scale), s.data_ptr(),
+                                           h.data_ptr(), out_state.data_ptr(), _current_stream(dev)),
+                   "ltc_gated_scan_step")
+    return h, out_state
+
+
+# ---------------------------------------------------------------------------
+# Losses and scores over a vocabulary
+# ---------------------------------------------------------------------------
+DISTILL_MAX_K = 256
+TOKEN_LOGPROBS_MAX_TOP = 64
+
+
+def _logits_operand(logits, temperature: float):
+    """(tensor with contiguous rows, its C description's fields).  Two strides describe the
+    rows, so slices like ``logits[:, :-1]`` are read where they lie."""
+    _typed(logits, "logits")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must be (..., V) with V >= 1, got shape {tuple(logits.shape)}")
+    if logits.shape[-1] > 1 << 30:
+        raise ValueError("the vocabulary has more than 2^30 entries")
+    if not 0.0 < temperature < 1e30:
+        raise ValueError(f"temperature must be positive (got {temperature})")
+    _on_cuda(logits, "logits")
+    z = _rows(logits)
+    lead = [(n, st) for n, st in zip(z.shape[:-1], z.stride()[:-1]) if n != 1]
+    merged = []  # outer to inner; neighbours that one stride walks are one
+    for n, st in lead:
+        if merged and merged[-1][1] == n * st:
+            merged[-1] = (merged[-1][0] * n, st)
+        else:
+            merged.append((n, st))
+    if len(merged) > 2:
+        z = z.contiguous()
+        merged = [(z.numel() // z.shape[-1], z.shape[-1])]
+    while len(merged) < 2:
+        merged.insert(0, (1, 0))
+    rows = merged[0][0] * merged[1][0]
+    return z, (rows, max(1, merged[1][0]), merged[0][1], merged[1][1], z.shape[-1], _DTYPES[z.dtype], temperature)
+
+
+def _id_operand(t, name: str, device, shape) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name} must be an int32 or int64 tensor")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return t.to(torch.int64).contiguous()
+
+
+def _row_grad(g: Optional[torch.Tensor], rows: int):
+    """(tensor, stride) of a per-row gradient; one that is the same for all rows stays a single value."""
+    if g is None:
+        return None, 0
+    g = g.to(torch.float32)
+    if rows > 1 and all(st == 0 or n == 1 for n, st in zip(g.shape, g.stride())):
+        return g, 0
+    return g.contiguous(), 1
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, ids, teacher, desc, needs_grad):
+        lib = _require_kernels()
+        dev, rows, K = z.device, desc[0], ids.shape[-1]
+        ctx.desc = desc
+        loss = torch.empty(z.shape[:-1], device=dev, dtype=torch.float32)
+        probs = torch.empty(rows, K, device=dev, dtype=torch.float32) if needs_grad else None
+        stats = torch.empty(rows, 4, device=dev, dtype=torch.float32) if needs_grad else None
+        if rows:
+            with torch.cuda.device(dev):
+                _check(lib.ltc_distill_forward(ctypes.byref(LtcLogits(z.data_ptr(), *desc)), ids.data_ptr(),
+                                               teacher.data_ptr(), _DTYPES[teacher.dtype], K, loss.data_ptr(),
+                                               _ptr(probs), _ptr(stats), _current_stream(dev)), "ltc_distill_loss")
+        if needs_grad:
+            ctx.save_for_backward(z, ids, probs, stats)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        lib = _require_kernels()
+        z, ids, probs, stats = ctx.saved_tensors
+        dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
+        g, stride = _row_grad(g, ctx.desc[0])
+        if ctx.desc[0]:
+            with torch.cuda.device(z.device):
+                _check(lib.ltc_distill_backward(ctypes.byref(LtcLogits(z.data_ptr(), *ctx.desc)), ids.data_ptr(),
+                                                ids.shape[-1], probs.data_ptr(), stats.data_ptr(), g.data_ptr(),
+                                                stride, dz.data_ptr(), _current_stream(z.device)),
+                       "ltc_distill_loss backward")
+        return dz, None, None, None, None
+
+
+def ltc_distill_loss(logits, teacher_ids, teacher_logits, temperature: float = 1.0) -> torch.Tensor:
+    """Distillation from a teacher's top entries -> fp32 losses ``logits.shape[:-1]``:
+
+    ``temperature**2 * sum_k p_k * (log p_k - log q[id_k])`` with ``q = softmax(logits /
+    temperature)`` over the vocabulary and ``p = softmax(teacher_logits / temperature)``
+    over the row's entries.
+
+    ``logits`` ``(..., V)`` fp32, bf16 or fp16; ``teacher_ids`` (int32 or int64) and
+    ``teacher_logits`` (logits or log probabilities, any of the three types) ``(..., K)``,
+    ``K <= 256``.  A negative id is no entry; a row without entries costs 0 and gets no
+    gradient; an id past the vocabulary makes its row NaN.  The gradient goes to ``logits``
+    alone (the teacher is a constant), once, rounded once to their type."""
+    z, desc = _logits_operand(logits, float(temperature))
+    _typed(teacher_logits, "teacher_logits", device=z.device)
+    shape = teacher_logits.shape
+    if tuple(shape[:-1]) != tuple(z.shape[:-1]) or not 1 <= (shape[-1] if len(shape) else 0) <= DISTILL_MAX_K:
+        raise ValueError(f"teacher_logits has shape {tuple(shape)}, expected {tuple(z.shape[:-1])} + (K,) "
+                         f"with 1 <= K <= {DISTILL_MAX_K}")
+    ids = _id_operand(teacher_ids, "teacher_ids", z.device, shape)
+    return _DistillLoss.apply(z, ids, teacher_logits.detach().contiguous(), desc, _wants_grad(z))
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: Optional[torch.Tensor]
+    top_logprobs: Optional[torch.Tensor]
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, tokens, desc, top_k, needs_grad):
+        lib = _require_kernels()
+        dev, rows, lead = z.device, desc[0], z.shape[:-1]
+        ctx.desc = desc
+        ctx.set_materialize_grads(False)
+        lp = torch.empty(lead, device=dev, dtype=torch.float32)
+        ent = torch.empty(lead, device=dev, dtype=torch.float32)
+        stats = torch.empty(rows, 4, device=dev, dtype=torch.float32) if needs_grad else None
+        top_ids = torch.empty(*lead, top_k, device=dev, dtype=torch.int64)
+        top_lp = torch.empty(*lead, top_k, device=dev, dtype=torch.float32)
+        if rows:
+            with torch.cuda.device(dev):
+                _check(lib.ltc_token_logprobs_forward(ctypes.byref(LtcLogits(z.data_ptr(), *desc)), tokens.data_ptr(),
+                                                      top_k, lp.data_ptr(), ent.data_ptr(), top_ids.data_ptr(),
+                                                      top_lp.data_ptr(), _ptr(stats), _current_stream(dev)),
+                       "ltc_token_logprobs")
+        if needs_grad:
+            ctx.save_for_backward(z, tokens, stats)
+        ctx.mark_non_differentiable(top_ids, top_lp)
+        return lp, ent, top_ids, top_lp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent, *_):
+        lib = _require_kernels()
+        z, tokens, stats = ctx.saved_tensors
+        rows = ctx.desc[0]
+        dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
+        g_lp, lp_stride = _row_grad(g_lp, rows)
+        g_ent, ent_stride = _row_grad(g_ent, rows)
+        if rows:
+            with torch.cuda.device(z.device):
+                _check(lib.ltc_token_logprobs_backward(ctypes.byref(LtcLogits(z.data_ptr(), *ctx.desc)),
+                                                       tokens.data_ptr(), stats.data_ptr(), _ptr(g_lp), lp_stride,
+                                                       _ptr(g_ent), ent_stride, dz.data_ptr(),
+                                                       _current_stream(z.device)), "ltc_token_logprobs backward")
+        return dz, None, None, None, None
+
+
+def ltc_token_logprobs(logits, tokens, top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+    """Log probability of each given token under ``softmax(logits / temperature)``, the
+    entropy of that distribution (nats), and its ``top_k <= 64`` best alternatives.
+
+    ``logits`` ``(..., V)`` fp32, bf16 or fp16, ``tokens`` ``(...)`` int32 or int64.  A negative
+    token is padding: log probability 0 and no gradient from it; one past the vocabulary
+    gives NaN.  ``top_ids`` / ``top_logprobs`` ``(..., top_k)`` are sorted, ties to the
+    lowest id (``None`` when ``top_k`` is 0); where fewer entries are above ``-inf`` they
+    hold -1 and ``-inf``.  A row of nothing but ``-inf`` has log probabilities ``-inf``,
+    entropy 0 and gradient 0.  Differentiable once in ``logits`` through ``logprobs`` and
+    ``entropy``."""
+    z, desc = _logits_operand(logits, float(temperature))
+    tok = _id_operand(tokens, "tokens", z.device, z.shape[:-1])
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(TOKEN_LOGPROBS_MAX_TOP, z.shape[-1]):
+        raise ValueError(f"top_k must be between 0 and min({TOKEN_LOGPROBS_MAX_TOP}, V) (got {top_k})")
+    lp, ent, ids, best = _TokenLogprobs.apply(z, tok, desc, top_k, _wants_grad(z))
+    return TokenLogprobs(lp, ent, ids if top_k else None, best if top_k else None)
