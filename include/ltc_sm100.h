@@ -222,12 +222,12 @@ typedef struct {
   int64_t stride_b, stride_t;
 } LtcScanInput;
 
-/* saved_bytes: state before each tile of `tile` tokens, kept by a forward for its backward
- * (0 when one tile covers a row).  segments: parts that time is cut into when there are
- * too few (sequence, channel) chains to fill the GPU. */
+/* saved_bytes: state before every 32nd token, kept by a forward for its backward (0 up to
+ * 32 tokens).  cluster: blocks that share one sequence x 32 channels where there are too few
+ * of those to fill the GPU. */
 typedef struct {
   size_t saved_bytes, fwd_workspace_bytes, bwd_workspace_bytes;
-  int32_t tile, segments;
+  int32_t cluster;
 } LtcScanPlan;
 
 int ltc_scan_plan(const LtcScanDims* dims, LtcScanPlan* out);

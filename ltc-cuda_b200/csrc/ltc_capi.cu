@@ -887,7 +887,7 @@ namespace {
 struct ScanCall {
   DeviceInfo di;
   ScanPlan plan;
-  size_t agg_floats, part_floats, saved_floats;
+  size_t part_floats, saved_floats;
 };
 
 int scan_begin(const LtcScanDims* d, const char* who, ScanCall* c) {
@@ -895,29 +895,27 @@ int scan_begin(const LtcScanDims* d, const char* who, ScanCall* c) {
   if (d->B < 1 || d->T < 1 || d->H < 1 || d->T > 0x7fffff00)
     return fail("%s: need B, T, H >= 1 (got %d, %d, %d)", who, d->B, d->T, d->H);
   if (d->dtype < 0 || d->dtype > LTC_DTYPE_F16) return fail("%s: unknown dtype %d", who, d->dtype);
+  if (d->H > kScanMaxH) return fail("%s: at most %d channels", who, kScanMaxH);
   if (d->num_seqs < 0 || (d->num_seqs > 0 && d->B != 1)) return fail("%s: packed sequences need B = 1", who);
   int err = 0;
   c->di = device_info(&err);
   if (err) return 1;
   c->plan = plan_scan(d->B, d->T, d->H, d->num_seqs > 0, c->di.sms);
   const size_t bh = (size_t)d->B * d->H;
-  c->agg_floats = c->plan.nseg > 1 ? bh * c->plan.nseg * 2 : 0;
-  c->part_floats = bh * c->plan.nseg;
-  c->saved_floats = c->plan.tiles > 1 ? bh * c->plan.tiles : 0;
+  c->part_floats = bh * c->plan.cl;
+  c->saved_floats = bh * c->plan.nbounds;
   return 0;
 }
 
-size_t scan_carve(const ScanCall& c, bool bwd, void* ws, ScanArgs* a) {
-  Carver k(ws);
-  float* agg = c.agg_floats ? k.take<float>(c.agg_floats) : nullptr;
-  int* cut = c.agg_floats ? k.take<int>(c.plan.nseg) : nullptr;
-  float* part = bwd ? k.take<float>(c.part_floats) : nullptr;
-  if (a) {
-    a->agg = agg;
-    a->seg_cut = cut;
-    a->part = part;
-  }
-  return k.off ? k.off + 256 : 0;
+// the forward needs no workspace
+size_t scan_workspace(const ScanCall& c, bool bwd) { return bwd ? c.part_floats * sizeof(float) : 0; }
+
+int scan_strides(const LtcScanDims* d, const char* who, const LtcScanInput* in, int i, ScanArgs* a) {
+  const int64_t bytes = in->stride_t * (d->dtype == LTC_DTYPE_F32 ? 4 : 2);
+  if (in->stride_t < -(1 << 28) || in->stride_t > (1 << 28)) return fail("%s: a time stride is past 2^28", who);
+  a->sb[i] = in->stride_b;
+  a->st[i] = (int)bytes;
+  return 0;
 }
 
 // inputs and everything the two directions share
@@ -926,18 +924,17 @@ int scan_args(const LtcScanDims* d, const ScanCall& c, const char* who, const Lt
   for (int i = 0; i < nin; ++i) {
     if (!in[i] || !in[i]->data) return fail("%s: input %d is NULL", who, i);
     a->in[i] = in[i]->data;
-    a->sb[i] = in[i]->stride_b;
-    a->st[i] = in[i]->stride_t;
+    if (scan_strides(d, who, in[i], i, a)) return 1;
   }
   if ((d->num_seqs > 0) != (starts != nullptr)) return fail("%s: num_seqs and seq_starts go together", who);
-  const size_t need = scan_carve(c, bwd, nullptr, nullptr);
+  const size_t need = scan_workspace(c, bwd);
   if (need > 0 && (!ws || ws_bytes < need))
     return fail("%s: workspace of %zu bytes is smaller than the %zu bytes required", who, ws ? ws_bytes : 0, need);
-  scan_carve(c, bwd, need ? ws : nullptr, a);
+  a->part = static_cast<float*>(ws);
   a->h0 = h0;
   a->starts = starts;
   a->B = d->B; a->T = d->T; a->H = d->H; a->S = d->num_seqs;
-  a->tile = c.plan.tile; a->tiles = c.plan.tiles; a->seg_tiles = c.plan.seg_tiles; a->nseg = c.plan.nseg;
+  a->nbounds = c.plan.nbounds; a->cl = c.plan.cl;
   return 0;
 }
 
@@ -981,8 +978,7 @@ int scan_backward(const LtcScanDims* d, const char* who, int policy, const LtcSc
   }
   if (dh && dh->data) {
     a.dh = dh->data;
-    a.sb[3] = dh->stride_b;
-    a.st[3] = dh->stride_t;
+    if (scan_strides(d, who, dh, 3, &a)) return 1;
   }
   a.decay = decay; a.scale = scale;
   a.bounds = const_cast<float*>(static_cast<const float*>(saved));
@@ -1033,10 +1029,9 @@ int ltc_scan_plan(const LtcScanDims* dims, LtcScanPlan* out) {
   ScanCall c;
   if (scan_begin(dims, "ltc_scan_plan", &c)) return 1;
   out->saved_bytes = c.saved_floats * sizeof(float);
-  out->fwd_workspace_bytes = scan_carve(c, false, nullptr, nullptr);
-  out->bwd_workspace_bytes = scan_carve(c, true, nullptr, nullptr);
-  out->tile = c.plan.tile;
-  out->segments = c.plan.nseg;
+  out->fwd_workspace_bytes = scan_workspace(c, false);
+  out->bwd_workspace_bytes = scan_workspace(c, true);
+  out->cluster = c.plan.cl;
   g_last_error.clear();
   return 0;
 }

@@ -207,37 +207,36 @@ cudaError_t launch_preamble_fwd(const PreambleArgs& a, int num_sms, cudaStream_t
 cudaError_t launch_preamble_bwd(const PreambleArgs& a, int num_sms, cudaStream_t st);
 
 // ---- linear recurrences over time (ltc_scan.cu) -----------------------------
-constexpr int kScanShortTile = 16, kScanLongTile = 64;  // tokens per tile
+constexpr int kScanShort = 16;       // rows up to this length are one tile of one warp
+constexpr int kScanBound = 32;       // the forward saves the state before every so many tokens
+constexpr int kScanMaxH = 1 << 28;   // channels, and time strides: byte offsets of a row fit 32 bits
+constexpr int kScanMaxCluster = 16;  // blocks that share one item (sequence x 32 channels)
 struct ScanArgs {
   const void* in[3];        // linear: a, b; gated: x, rate, gate
   const void* dh;           // gradient of h (backward) or null
-  long long sb[4], st[4];   // batch and time strides (elements) of in[0..2] and dh; channels are contiguous
+  long long sb[4];          // batch strides (elements) of in[0..2] and dh; channels are contiguous
+  int st[4];                // their time strides (bytes)
   const float* decay;       // (H), gated
   const float* h0;          // (B or S, H) or null (zeros)
   const float* dhT;         // gradient of the final state, (B or S, H) or null
   const int* starts;        // (S+1) token offsets of packed sequences (B = 1) or null
   void* h;                  // (B,T,H)
   float* hT;                // (B or S, H)
-  float* bounds;            // (B, tiles, H) state before each tile; null when no backward follows
+  float* bounds;            // (B, nbounds, H) state before tokens 32, 64, ..; null when no backward follows
   void* d[3];               // gradients of in[]
   float* dh0;               // (B or S, H) or null
   float* ddecay;            // (H), gated
-  float* agg;               // (B, nseg, 2, H) folds of the segments (nseg > 1)
-  int* seg_cut;             // (nseg) packed: whether the segment holds a sequence start
-  float* part;              // (B, nseg, H) partial decay gradients
+  float* part;              // (B, cl, H) partial decay gradients
   int B, T, H, S;
   float scale;
-  int tile, tiles, seg_tiles, nseg;  // ScanPlan
+  int nbounds, cl;          // ScanPlan
   // set per launch
-  int chb, launch_segs;
+  int chb, rounds;          // items side by side; tiles a block walks
   long long items;
-  bool fold_only;
 };
 struct ScanPlan {
-  int tile;       // tokens per tile
-  int tiles;      // tiles of a row
-  int seg_tiles;  // tiles of a segment
-  int nseg;       // segments of a row
+  int nbounds;  // saved states of a row
+  int cl;       // blocks of an item
 };
 ScanPlan plan_scan(int B, int T, int H, bool packed, int num_sms);
 // policy 0: linear, 1: gated; dtype 0: fp32, 1: bf16, 2: fp16
@@ -271,6 +270,7 @@ struct VocabArgs {
   void* dz;                  // (rows, V)
   // set per launch
   int cluster, chunk, chunks;
+  long long blocks;          // rows at work at a time (forward)
 };
 cudaError_t launch_vocab_fwd(VocabArgs a, int dtype, bool distill, int num_sms, cudaStream_t st);
 cudaError_t launch_vocab_bwd(VocabArgs a, int dtype, bool distill, cudaStream_t st);

@@ -7,43 +7,48 @@
 // Mathematics.  A run of tokens maps the state before it to the state behind it,
 // h -> A h + B, and two runs compose as (A2 A1, A2 B1 + B2).  With c_t = a_t lambda_t the
 // adjoint lambda_t = dh_t + a_{t+1} lambda_{t+1} runs backwards by the same kind of map,
-// c -> A c + B with B folded from the far end, over the SAME product A.
+// c -> A c + C with C folded from the far end, over the SAME product A.
 //
-// Work split.  A tile is TY x R tokens by LX x VEC channels: a thread keeps R consecutive
-// tokens of VEC channels in registers, folds them to one (A, B), the fold is combined
-// over the tile's TY threads (shuffles inside a warp, shared memory across warps, one
-// barrier per tile), and the thread then runs its tokens again from its own first state.
-// A group of threads marches over its tiles with the state in registers, so every input
-// is read once.  Where there are too few (sequence, channel) chains to fill the GPU, time
-// is cut into segments: a first launch folds each segment to (A, B), the second starts
-// each segment from the fold of the earlier ones (fixed order: results do not depend on
-// scheduling; nothing waits inside a kernel).
+// Work split.  An item is one sequence x 32 channels.  A tile is TY x R tokens of it: a
+// thread keeps R consecutive tokens of VEC channels in registers, folds them to one (A, B),
+// the folds are combined over the tile's TY threads (a shuffle inside a warp, shared memory
+// across warps), and the thread runs its tokens again from its own first state.  A group of
+// threads marches over its tiles with the state in registers, so every input is read once;
+// the next tile's loads are in flight while this one is combined and written.  Where there
+// are too few items to fill the GPU, a cluster of up to 16 blocks takes one item, block r the
+// tiles r, r + cl, ...: the blocks' folds go to every block's shared memory, one cluster
+// barrier per round.  All orders are fixed: results do not depend on scheduling.
 //
-// Backward.  The forward leaves the state before each tile (fp32, one row in 16 or 64
-// tokens); the backward rebuilds the states of a tile from it in registers instead of
-// reading h, which is both one tensor less and exact where h was rounded to 16 bits.
+// Backward.  The forward leaves the state before every 32nd token (fp32); the backward
+// rebuilds the states of a tile from it in registers instead of reading h, which is both
+// one tensor less and exact where h was rounded to 16 bits.
 //
 // Packed sequences: token t that starts sequence n is a cut, h_t = a_t h0[n] + b_t whatever came
-// before, and a run that holds one is a constant map; tokens outside every sequence give h = 0 and zero gradients.
+// before, and a run that holds one is a constant map; tokens outside every sequence give
+// h = 0 and zero gradients.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "ltc_common.cuh"
 #include "ltc_internal.h"
 
+namespace cg = cooperative_groups;
+
 namespace ltc {
 
 namespace {
 
 constexpr int kThreads = 128;
+constexpr int kItem = 32;  // channels of an item: LX * VEC in every variant
 
 // ---- element types -------------------------------------------------------------
 template <typename T, int VEC> struct Raw;  // VEC elements as loaded
-template <> struct Raw<float, 4> { using type = float4; };
+template <> struct Raw<float, 2> { using type = float2; };
 template <> struct Raw<float, 1> { using type = float; };
-template <> struct Raw<__nv_bfloat16, 4> { using type = uint2; };
+template <> struct Raw<__nv_bfloat16, 2> { using type = unsigned; };
 template <> struct Raw<__nv_bfloat16, 1> { using type = unsigned short; };
-template <> struct Raw<__half, 4> { using type = uint2; };
+template <> struct Raw<__half, 2> { using type = unsigned; };
 template <> struct Raw<__half, 1> { using type = unsigned short; };
 
 __device__ __forceinline__ float2 up2(unsigned v, __nv_bfloat16) {
@@ -61,96 +66,127 @@ __device__ __forceinline__ unsigned down2(float x, float y, __half) {
   return *reinterpret_cast<unsigned*>(&p);
 }
 
-__device__ __forceinline__ void unpack(const float4& r, float (&v)[4], float) {
-  v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
-}
-template <typename T>
-__device__ __forceinline__ void unpack(const uint2& r, float (&v)[4], T) {
-  const float2 lo = up2(r.x, T()), hi = up2(r.y, T());
-  v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
-}
-__device__ __forceinline__ void unpack(const float& r, float (&v)[1], float) { v[0] = r; }
-template <typename T>
-__device__ __forceinline__ void unpack(const unsigned short& r, float (&v)[1], T) {
-  v[0] = up2(r, T()).x;
-}
+// The channels of one token that a thread holds: one, or two in packed fp32 instructions.
+template <int VEC> struct Chans;
+template <> struct Chans<1> { using type = float; };
+template <> struct Chans<2> { using type = float2; };
 
-__device__ __forceinline__ void store(float* p, const float (&v)[4]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-}
-__device__ __forceinline__ void store(float* p, const float (&v)[1]) { *p = v[0]; }
-template <typename T>
-__device__ __forceinline__ void store(T* p, const float (&v)[4]) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(down2(v[0], v[1], T()), down2(v[2], v[3], T()));
-}
-template <typename T>
-__device__ __forceinline__ void store(T* p, const float (&v)[1]) {
-  *reinterpret_cast<unsigned short*>(p) = (unsigned short)(down2(v[0], 0.f, T()) & 0xffffu);
-}
-__device__ __forceinline__ void load_f32(const float* p, float (&v)[4]) {
-  const float4 r = *reinterpret_cast<const float4*>(p);
-  v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
-}
-__device__ __forceinline__ void load_f32(const float* p, float (&v)[1]) { v[0] = *p; }
+__device__ __forceinline__ float vfma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 vfma(float2 a, float2 b, float2 c) { return fma2(a, b, c); }
+__device__ __forceinline__ float vmul(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 vmul(float2 a, float2 b) { return mul2(a, b); }
+__device__ __forceinline__ float vadd(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 vadd(float2 a, float2 b) { return add2(a, b); }
+template <typename V> __device__ __forceinline__ V all_of(float x);
+template <> __device__ __forceinline__ float all_of<float>(float x) { return x; }
+template <> __device__ __forceinline__ float2 all_of<float2>(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 two(float x) { return make_float2(x, x); }
+template <typename F> __device__ __forceinline__ float vmap(float x, F f) { return f(x); }
+template <typename F> __device__ __forceinline__ float2 vmap(float2 x, F f) { return make_float2(f(x.x), f(x.y)); }
+// lane exchange
+__device__ __forceinline__ float vxor(float v, int d) { return __shfl_xor_sync(0xffffffffu, v, d); }
+__device__ __forceinline__ float2 vxor(float2 v, int d) { return make_float2(vxor(v.x, d), vxor(v.y, d)); }
 
+__device__ __forceinline__ void unpack(const float2& r, float2& v, float) { v = r; }
+__device__ __forceinline__ void unpack(const float& r, float& v, float) { v = r; }
+template <typename T>
+__device__ __forceinline__ void unpack(const unsigned& r, float2& v, T) { v = up2(r, T()); }
+template <typename T>
+__device__ __forceinline__ void unpack(const unsigned short& r, float& v, T) { v = up2(r, T()).x; }
+
+__device__ __forceinline__ void store(float* p, float2 v) { *reinterpret_cast<float2*>(p) = v; }
+__device__ __forceinline__ void store(float* p, float v) { *p = v; }
+template <typename T>
+__device__ __forceinline__ void store(T* p, float2 v) { *reinterpret_cast<unsigned*>(p) = down2(v.x, v.y, T()); }
+template <typename T>
+__device__ __forceinline__ void store(T* p, float v) {
+  *reinterpret_cast<unsigned short*>(p) = (unsigned short)(down2(v, 0.f, T()) & 0xffffu);
+}
+template <typename T, typename C>
+__device__ __forceinline__ T* at(C* p, int j, int bytes) {
+  return reinterpret_cast<T*>(p + (long long)j * bytes);
+}
+template <typename V>
+__device__ __forceinline__ V load_f32(const float* p) { return *reinterpret_cast<const V*>(p); }
 template <typename T, int VEC>
-__device__ __forceinline__ typename Raw<T, VEC>::type load_raw(const void* base, long long off, bool ok) {
-  using V = typename Raw<T, VEC>::type;
-  V r{};
-  if (ok) r = __ldg(reinterpret_cast<const V*>(static_cast<const T*>(base) + off));
-  return r;
+__device__ __forceinline__ typename Raw<T, VEC>::type load_raw(const T* p) {
+  return __ldg(reinterpret_cast<const typename Raw<T, VEC>::type*>(p));
 }
 
 // ---- gates ---------------------------------------------------------------------
-// fp32 inputs take the library's expf; 16-bit inputs __expf (2 ulp plus the rounding of
-// its argument, far below the inputs' own 2^-9)
-template <typename T> __device__ __forceinline__ float exp_of(float x) { return __expf(x); }
-template <> __device__ __forceinline__ float exp_of<float>(float x) { return expf(x); }
+// On two elements at a time, in packed fp32 instructions.  The hardware's exp2, reciprocal
+// and reciprocal root are off by about 2 ulp each, which leaves the results where a chain of
+// correctly rounded operations has them (the tests' bounds count it).  With cu = scale
+// softplus(decay) log2(e):  a = 2^-u,  u = cu sigmoid(rate) >= 0.
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kTinyOm = 1e-36f;  // keeps 1 / (1 - a^2) finite; b is 0 long before
 
-template <typename T>
-__device__ __forceinline__ float sigmoid_of(float x) { return rcp_approx(1.f + exp_of<T>(-x)); }
-
-// 1 - exp(y), y <= 0.  Near 0, where 1 - exp(y) cancels, the Taylor series of
-// -(exp(y) - 1), whose first left-out term is below 2^-24 of the sum for y > -1/4; past
-// it 1 - e is at least 0.22.
-__device__ __forceinline__ float one_minus_exp(float y, float e) {
-  float p = fmaf(y, 1.f / 720.f, 1.f / 120.f);
-  p = fmaf(y, p, 1.f / 24.f);
-  p = fmaf(y, p, 1.f / 6.f);
-  p = fmaf(y, p, 0.5f);
-  p = fmaf(y, p, 1.f);
-  return y > -0.25f ? -y * p : 1.f - e;
-}
-
-__device__ __forceinline__ float sqrt_approx(float x) {
+__device__ __forceinline__ float ex2(float x) {
   float y;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float rsqrt_ftz(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 ex2_2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
+__device__ __forceinline__ float2 rcp_2(float2 x) { return make_float2(rcp_approx(x.x), rcp_approx(x.y)); }
+
+// 1 - a^2 = 1 - exp(-y), y = 2 ln(2) u.  Near 0, where the difference cancels, the Taylor
+// series y - y^2/2 + ... in u, whose first left-out term is below 2^-24 of the sum for
+// y < 1/4; past it 1 - a^2 is at least 0.22.
+__device__ __forceinline__ float2 one_minus_sq(float2 a, float2 u) {
+  constexpr double c = 1.3862943611198906;  // 2 ln 2
+  float2 p = fma2(u, two((float)(-c * c * c * c * c * c / 720)), two((float)(c * c * c * c * c / 120)));
+  p = fma2(u, p, two((float)(-c * c * c * c / 24)));
+  p = fma2(u, p, two((float)(c * c * c / 6)));
+  p = fma2(u, p, two((float)(-c * c / 2)));
+  p = mul2(fma2(u, p, two((float)c)), u);
+  constexpr float limit = (float)(0.25 / c);
+  return make_float2(u.x < limit ? p.x : fmaf(-a.x, a.x, 1.f), u.y < limit ? p.y : fmaf(-a.y, a.y, 1.f));
 }
 
 __device__ __forceinline__ float softplus_of(float x) { return x > 20.f ? x : log1pf(expf(x)); }
+__device__ __forceinline__ float sigmoid_of(float x) { return 1.f / (1.f + expf(-x)); }
+__device__ __forceinline__ float rate_of(float decay, float scale) { return scale * softplus_of(decay) * kLog2e; }
 
-struct Gate {
-  float sr, sg, a, beta;
-};
-// cs = -scale * softplus(decay)
-template <typename T>
-__device__ __forceinline__ Gate gate_of(float rate, float gate, float cs) {
-  Gate g;
-  g.sr = sigmoid_of<T>(rate);
-  g.sg = sigmoid_of<T>(gate);
-  const float L = cs * g.sr;
-  g.a = exp_of<T>(L);
-  g.beta = sqrt_approx(one_minus_exp(2.f * L, g.a * g.a));
-  return g;
+// a, and w = sqrt(1 - a^2) sigmoid(gate) as (1 - a^2) rsqrt((1 - a^2) (1 + exp(-gate))^2): one
+// instruction for the root and the reciprocal (a gate below -44 overflows the square and
+// gives 0 instead of its 1e-19)
+__device__ __forceinline__ void gate_fwd(float2 rate, float2 gate, float2 cu, float2& a, float2& w) {
+  const float2 s = rcp_2(add2(ex2_2(mul2(rate, two(-kLog2e))), two(1.f)));
+  const float2 u = mul2(cu, s);
+  a = make_float2(ex2(-u.x), ex2(-u.y));
+  const float2 om = one_minus_sq(a, u);
+  const float2 pg = add2(ex2_2(mul2(gate, two(-kLog2e))), two(1.f));
+  const float2 q = mul2(mul2(make_float2(fmaxf(om.x, kTinyOm), fmaxf(om.y, kTinyOm)), pg), pg);
+  w = mul2(om, make_float2(rsqrt_ftz(q.x), rsqrt_ftz(q.y)));
+}
+// the same with what the gradients need: s = sigmoid(rate), b = w x,
+// k = -b a^2 / (1 - a^2) (dL/dL_t = lambda (a h_{t-1} + k)), m = b (1 - sigmoid(gate))
+__device__ __forceinline__ void gate_bwd(float2 x, float2 rate, float2 gate, float2 cu, float2& a, float2& w,
+                                         float2& s, float2& b, float2& k, float2& m) {
+  s = rcp_2(add2(ex2_2(mul2(rate, two(-kLog2e))), two(1.f)));
+  const float2 u = mul2(cu, s);
+  a = make_float2(ex2(-u.x), ex2(-u.y));
+  const float2 om = one_minus_sq(a, u);
+  const float2 sg = rcp_2(add2(ex2_2(mul2(gate, two(-kLog2e))), two(1.f)));
+  const float2 rs = make_float2(rsqrt_ftz(fmaxf(om.x, kTinyOm)), rsqrt_ftz(fmaxf(om.y, kTinyOm)));
+  w = mul2(mul2(om, rs), sg);
+  b = mul2(w, x);
+  const float2 ar = mul2(a, rs), nb = mul2(b, two(-1.f));
+  k = mul2(mul2(nb, ar), ar);
+  m = fma2(nb, sg, b);
 }
 
 // h -> a h + b, or b behind a cut: where a packed sequence starts, whatever the earlier one
 // holds stops there, infinities and NaN too, which a zero factor would let through.  (An
 // underflown product is no cut: a NaN goes on through it as in the definition.)
-template <bool PACKED>
-__device__ __forceinline__ float flow(bool cut, float a, float h, float b) {
-  return PACKED && cut ? b : fmaf(a, h, b);
+template <bool PACKED, typename V>
+__device__ __forceinline__ V flow(bool cut, V a, V h, V b) {
+  return PACKED && cut ? b : vfma(a, h, b);
 }
 
 // ---- packed sequences ------------------------------------------------------------
@@ -168,618 +204,701 @@ struct Marks {         // of a thread's R tokens, one bit each
   unsigned first = 0;  // starts its sequence
   unsigned last = 0;   // ends it
   unsigned out = 0;    // belongs to none
-  int n0 = 0;          // sequence of the first token
+  int nf = 0, nl = 0;  // sequences of the earliest first and of the earliest last one
 };
-template <int R>
-__device__ __forceinline__ Marks marks_of(const int* starts, int S, int t0, int T) {
-  Marks m;
-  m.n0 = seq_of(starts, S, t0);
-  const int end = min(__ldg(starts + S), T), begin = __ldg(starts);
-  int n = m.n0, s0 = __ldg(starts + n), s1 = __ldg(starts + n + 1);
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int t = t0 + j;
-    while (t >= s1 && n + 1 < S) {
-      ++n;
-      s0 = s1;
-      s1 = __ldg(starts + n + 1);
-    }
-    const bool in = t >= begin && t < end;
-    m.out |= (in ? 0u : 1u) << j;
-    m.first |= (in && t == s0 ? 1u : 0u) << j;
-    m.last |= (in && t + 1 == s1 ? 1u : 0u) << j;
-  }
-  return m;
+// the sequence that token t0 + j starts or ends
+__device__ __forceinline__ int seq_at(unsigned bits, int n, int j, const int* starts, int S, int t0) {
+  return bits & ((1u << j) - 1) ? seq_of(starts, S, t0 + j) : n;
 }
 
-// ---- one tile's fold over the threads of a group -----------------------------------
-// NF forward folds and NR reverse folds share the product A.  LX lanes hold different
-// channels; the TY threads with the same channels hold consecutive tokens.
-template <int LX, int TY>
-struct Geo {
-  static constexpr int GPW = 32 / LX;       // time groups inside a warp
-  static constexpr int NW = TY / GPW > 0 ? TY / GPW : 1;  // warps along time
-  static_assert(TY % GPW == 0, "a warp's time groups belong to one tile");
+// Where a warp's tiles lie among the sequences.  Each lane keeps one of 32 evenly spread
+// offsets, so that finding a tile's sequence takes one load (more past 1024 sequences)
+// instead of a bisection's chain of them; nothing is looked up while the tiles stay inside
+// one sequence.
+struct Walk {
+  const int* starts;
+  int S, stride, pick, begin, end;
+  int n = 0, s0 = 0, s1 = 0;  // sequence of the last tile, its tokens [s0, s1)
+
+  __device__ __forceinline__ Walk(const int* starts_, int S_, int T) : starts(starts_), S(S_) {
+    stride = (S + 31) / 32;
+    const int at = (int)(threadIdx.x & 31) * stride;
+    pick = at < S ? __ldg(starts + at) : 0x7fffffff;
+    begin = __ldg(starts);
+    end = min(__ldg(starts + S), T);
+  }
+  // all lanes of a warp call it with the same tile
+  __device__ __forceinline__ void find(int t) {
+    const int block = max(__popc(__ballot_sync(0xffffffffu, pick <= t)) - 1, 0) * stride;
+    int count = 0;
+    for (int k = 0; k < stride; k += 32) {
+      const int at = block + k + (int)(threadIdx.x & 31);
+      const bool le = at < min(block + stride, S) && __ldg(starts + min(at, S)) <= t;
+      count += __popc(__ballot_sync(0xffffffffu, le));
+    }
+    n = min(block + max(count - 1, 0), S - 1);
+    s0 = __ldg(starts + n);
+    s1 = __ldg(starts + n + 1);
+  }
+  template <int R, int TT>
+  __device__ __forceinline__ Marks marks(int tile_t0, int t0) {
+    Marks m;
+    if (!(s0 < tile_t0 && tile_t0 < s1)) find(tile_t0);
+    if (s0 < tile_t0 && s1 > tile_t0 + TT && begin <= tile_t0 && end >= tile_t0 + TT) return m;
+    int k = n, a = s0, b = s1;
+#pragma unroll 1
+    for (int j = 0; j < R; ++j) {
+      const int t = t0 + j;
+      while (t >= b && k + 1 < S) {
+        ++k;
+        a = b;
+        b = __ldg(starts + k + 1);
+      }
+      const bool in = t >= begin && t < end;
+      if (!in) m.out |= 1u << j;
+      if (in && t == a) {
+        if (!m.first) m.nf = k;
+        m.first |= 1u << j;
+      }
+      if (in && t + 1 == b) {
+        if (!m.last) m.nl = k;
+        m.last |= 1u << j;
+      }
+    }
+    return m;
+  }
+};
+struct NoWalk {
+  __device__ __forceinline__ NoWalk(const int*, int, int) {}
+  template <int R, int TT>
+  __device__ __forceinline__ Marks marks(int, int) { return Marks{}; }
+};
+template <bool PACKED> struct WalkOf { using type = NoWalk; };
+template <> struct WalkOf<true> { using type = Walk; };
+
+// ---- shapes ----------------------------------------------------------------------
+template <int VEC_, int R_, int TY_, int BB_>
+struct Shape {
+  static constexpr int VEC = VEC_, R = R_, TY = TY_, BB = BB_;
+  static constexpr int LX = kItem / VEC;  // lanes side by side: one row of an item
+  static constexpr int GPW = 32 / LX;     // time groups inside a warp
+  static constexpr int NW = TY / GPW;     // warps along time
+  static constexpr int TT = TY * R;       // tokens of a tile
+  static constexpr int THREADS = LX * TY * BB;
+  static_assert(TY % GPW == 0 && THREADS % 32 == 0, "whole warps along time");
+  static_assert(BB == 1 || NW == 1, "several items per block only without block barriers");
+  static_assert((R * VEC) % 2 == 0 && GPW <= 2, "pairs; one shuffle step");
 };
 
-// ---- forward -----------------------------------------------------------------------
-template <int P, typename T, int VEC, int LX, int TY, int R, int BB, bool PACKED>
-__global__ void __launch_bounds__(kThreads) scan_fwd_kernel(ScanArgs g) {
-  using G = Geo<LX, TY>;
-  static_assert(LX * TY * BB == kThreads, "block shape");
-  static_assert(BB == 1 || G::NW == 1, "several items per block only without block barriers");
-  static_assert(!PACKED || G::NW > 1, "the one-warp tiles do not look at cuts");
-  constexpr int NIN = P ? 3 : 2;
-  constexpr int TT = TY * R;
-  __shared__ float sA[2][G::NW][LX * VEC], sB[2][G::NW][LX * VEC];
-  __shared__ int sF[2][G::NW];
-  const int lane = threadIdx.x & 31;
-  const int lx = threadIdx.x % LX, ty = (threadIdx.x / LX) % TY;
-  const int grp = ty % G::GPW, wt = ty / G::GPW;  // group in the warp, warp along time
-  const long long item = (long long)blockIdx.x * BB + threadIdx.x / (LX * TY);
-  if (BB > 1 && item >= g.items) return;  // whole warps leave; no block barrier follows
-  const int cb = (int)(item % g.chb);
-  const long long rest = item / g.chb;
-  const int seg = (int)(rest % g.launch_segs);
-  const long long b = rest / g.launch_segs;
-  const int ch = cb * LX * VEC + lx * VEC;
-  const bool chok = ch < g.H;
-  const int tile0 = seg * g.seg_tiles, tile1 = min(tile0 + g.seg_tiles, g.tiles);
+// what the blocks of a cluster tell each other about one round, and the warps of a block
+template <int NW, int NF>
+struct alignas(16) Exchange {
+  float w[2][NW][NF][kItem];   // per warp: A, then B (and C in the backward)
+  int wf[2][NW];               // whether it holds a cut
+  float x[2][kScanMaxCluster][2][kItem];  // per block: A and B or C
+  int xf[2][kScanMaxCluster];
+};
 
-  float cs[VEC];
+// sends this block's fold (over its warps, in time order) to all blocks of the cluster, and waits for theirs
+template <bool PACKED, bool REVERSE, int NW, int NF>
+__device__ __forceinline__ void exchange(Exchange<NW, NF>& sh, int buf, int cl, int rank) {
+  __syncthreads();
+  if (cl == 1) return;
+  cg::cluster_group c = cg::this_cluster();
+  if (threadIdx.x < kItem) {
+    const int ch = threadIdx.x;
+    float A = 1.f, B = 0.f;
+    int F = 0;
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) cs[v] = 0.f;
-  if (P && chok) {
-    load_f32(g.decay + ch, cs);
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) cs[v] = -g.scale * softplus_of(cs[v]);
-  }
-
-  // state before the segment; in the folding launch (0, 1) so that carry and prod become B and A
-  float carry[VEC], prod[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) { carry[v] = 0.f; prod[v] = 1.f; }
-  bool cut_all = false;
-  if (!g.fold_only && chok) {
-    if (!PACKED && g.h0) load_f32(g.h0 + b * g.H + ch, carry);
-    const float* ag = g.agg + (b * g.nseg * 2) * (long long)g.H + ch;
-    for (int s = 0; s < seg; ++s, ag += 2 * (long long)g.H) {
-      float fa[VEC], fb[VEC];
-      load_f32(ag, fa);
-      load_f32(ag + g.H, fb);
-      const bool cut = PACKED && g.seg_cut[s] != 0;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) carry[v] = flow<PACKED>(cut, fa[v], carry[v], fb[v]);
+    for (int i = 0; i < NW; ++i) {
+      const int w = REVERSE ? NW - 1 - i : i;
+      const float wa = sh.w[buf][w][0][ch];
+      const bool cut = PACKED && sh.wf[buf][w] != 0;
+      B = flow<PACKED>(cut, wa, B, sh.w[buf][w][NF - 1][ch]);
+      A *= wa;
+      F |= cut;
+    }
+    for (int r = 0; r < cl; ++r) {
+      Exchange<NW, NF>* to = c.map_shared_rank(&sh, r);
+      to->x[buf][rank][0][ch] = A;
+      to->x[buf][rank][1][ch] = B;
+      if (PACKED && ch == 0) to->xf[buf][rank] = F;
     }
   }
+  c.sync();
+}
 
-  for (int tile = tile0; tile < tile1; ++tile) {
-    const int t0 = tile * TT + ty * R;
-    typename Raw<T, VEC>::type raw[NIN][R];
+struct Item {
+  long long b;
+  int ch, rank;
+  bool chok;
+};
+template <typename S>
+__device__ __forceinline__ Item item_of(const ScanArgs& g, bool& out) {
+  Item it;
+  long long i = (long long)blockIdx.x;
+  it.rank = 0;
+  if (S::BB > 1) {
+    i = i * S::BB + threadIdx.x / (S::LX * S::TY);
+  } else if (g.cl > 1) {
+    it.rank = (int)(i % g.cl);
+    i /= g.cl;
+  }
+  out = S::BB > 1 && i >= g.items;
+  it.b = i / g.chb;
+  it.ch = (int)(i % g.chb) * kItem + (int)(threadIdx.x % S::LX) * S::VEC;
+  it.chok = it.ch < g.H;
+  return it;
+}
+
+// One tensor's R elements (or pairs) of a thread.  Byte addresses with a 32-bit byte stride:
+// one multiply-add each.  BRANCH: a whole run of tokens takes a path without tests, which the
+// forward gains from (88 against 92 us at 8 x 2048 x 2560 bf16) and the backward does not (201, 196).
+template <bool BRANCH, typename T, int VEC, int R>
+__device__ __forceinline__ void fetch_run(typename Raw<T, VEC>::type (&raw)[R], const char* p, int st, int left) {
+  if (BRANCH && left >= R) {
 #pragma unroll
-    for (int i = 0; i < NIN; ++i)
+    for (int j = 0; j < R; ++j) raw[j] = load_raw<T, VEC>(at<const T>(p, j, st));
+  } else {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      raw[j] = typename Raw<T, VEC>::type{};
+      if (j < left) raw[j] = load_raw<T, VEC>(at<const T>(p, j, st));
+    }
+  }
+}
+
+// A and B of a run of tokens
+template <bool PACKED, typename V, int R>
+__device__ __forceinline__ void fold_run(unsigned cuts, const V (&a)[R], const V (&b)[R], V& A, V& B) {
+  A = all_of<V>(1.f);
+  B = V{};
+  if (PACKED && cuts) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      B = flow<true>((cuts >> j) & 1u, a[j], B, b[j]);
+      A = vmul(A, a[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      B = vfma(a[j], B, b[j]);
+      A = vmul(A, a[j]);
+    }
+  }
+}
+
+// gates of a thread's elements: pairs of channels, or of tokens where it holds one channel
+template <int R>
+__device__ __forceinline__ void gates_fwd(const float2 (&x)[R], const float2 (&y)[R], const float2 (&z)[R], float2 cu,
+                                          float2 (&a)[R], float2 (&b)[R]) {
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    float2 w;
+    gate_fwd(y[j], z[j], cu, a[j], w);
+    b[j] = mul2(w, x[j]);
+  }
+}
+template <int R>
+__device__ __forceinline__ void gates_fwd(const float (&x)[R], const float (&y)[R], const float (&z)[R], float cu,
+                                          float (&a)[R], float (&b)[R]) {
+#pragma unroll
+  for (int j = 0; j < R; j += 2) {
+    float2 fa, fw;
+    gate_fwd(make_float2(y[j], y[j + 1]), make_float2(z[j], z[j + 1]), two(cu), fa, fw);
+    fw = mul2(fw, make_float2(x[j], x[j + 1]));
+    a[j] = fa.x; a[j + 1] = fa.y;
+    b[j] = fw.x; b[j + 1] = fw.y;
+  }
+}
+template <int R>
+__device__ __forceinline__ void gates_bwd(const float2 (&x)[R], const float2 (&y)[R], const float2 (&z)[R], float2 cu,
+                                          float2 (&a)[R], float2 (&w)[R], float2 (&s)[R], float2 (&b)[R],
+                                          float2 (&k)[R], float2 (&m)[R]) {
+#pragma unroll
+  for (int j = 0; j < R; ++j) gate_bwd(x[j], y[j], z[j], cu, a[j], w[j], s[j], b[j], k[j], m[j]);
+}
+template <int R>
+__device__ __forceinline__ void gates_bwd(const float (&x)[R], const float (&y)[R], const float (&z)[R], float cu,
+                                          float (&a)[R], float (&w)[R], float (&s)[R], float (&b)[R], float (&k)[R],
+                                          float (&m)[R]) {
+#pragma unroll
+  for (int j = 0; j < R; j += 2) {
+    float2 fa, fw, fs, fb, fk, fm;
+    gate_bwd(make_float2(x[j], x[j + 1]), make_float2(y[j], y[j + 1]), make_float2(z[j], z[j + 1]), two(cu), fa, fw,
+             fs, fb, fk, fm);
+    a[j] = fa.x; a[j + 1] = fa.y;
+    w[j] = fw.x; w[j + 1] = fw.y;
+    s[j] = fs.x; s[j + 1] = fs.y;
+    b[j] = fb.x; b[j + 1] = fb.y;
+    k[j] = fk.x; k[j + 1] = fk.y;
+    m[j] = fm.x; m[j + 1] = fm.y;
+  }
+}
+
+// ---- forward -----------------------------------------------------------------------
+template <int P, typename T, typename S, bool PACKED>
+__global__ void __launch_bounds__(S::THREADS, PACKED || (P && (sizeof(T) == 4 || S::VEC == 1)) ? 4 : 5) scan_fwd_kernel(ScanArgs g) {
+  static_assert(!PACKED || S::NW > 1, "the one-warp tiles do not look at cuts");
+  constexpr int NIN = P ? 3 : 2, VEC = S::VEC, R = S::R, NW = S::NW, LX = S::LX;
+  using V = typename Chans<VEC>::type;
+  __shared__ Exchange<NW, 2> sh;
+  const int lx = threadIdx.x % LX, ty = (threadIdx.x / LX) % S::TY;
+  const int grp = ty % S::GPW, wt = ty / S::GPW;  // group in the warp, warp along time
+  bool out_of_items;
+  const Item it = item_of<S>(g, out_of_items);
+  if (out_of_items) return;  // whole warps leave; no block barrier follows
+  const long long b = it.b;
+  const int ch = it.ch, cl = S::BB > 1 ? 1 : g.cl;
+  const bool chok = it.chok;
+  const int cr = chok ? ch : 0;  // lanes past the last channel read the first one and write nothing
+
+  V cu{}, carry{};  // carry: state before the round
+  if (P) cu = vmap(load_f32<V>(g.decay + cr), [&](float d) { return rate_of(d, g.scale); });
+  if (!PACKED && g.h0) carry = load_f32<V>(g.h0 + b * g.H + cr);
+
+  if (cl > 1) cg::this_cluster().sync();  // every block of the cluster runs before its memory is written
+  int t0 = it.rank * S::TT + ty * R;
+  const char* in[NIN];
+  typename Raw<T, VEC>::type raw[NIN][R];
+#pragma unroll
+  for (int i = 0; i < NIN; ++i) {
+    in[i] = reinterpret_cast<const char*>(static_cast<const T*>(g.in[i]) + b * g.sb[i] + cr) + (long long)t0 * g.st[i];
+    fetch_run<true, T, VEC, R>(raw[i], in[i], g.st[i], g.T - t0);
+  }
+  const int row = g.H * (int)sizeof(T);
+  char* out = reinterpret_cast<char*>(static_cast<T*>(g.h) + (b * g.T + t0) * g.H + ch);
+
+  // packed: marks and the first state that the tile needs, found while the tile before is at work
+  typename WalkOf<PACKED>::type walk(g.starts, g.S, g.T);
+  Marks m = walk.template marks<R, S::TT>(t0 - ty * R, t0);
+  V hz{};
+  if (PACKED && m.first && g.h0) hz = load_f32<V>(g.h0 + (long long)m.nf * g.H + cr);
+  for (int round = 0; round < g.rounds; ++round, t0 += cl * S::TT) {
+    const unsigned cuts = PACKED ? m.first | m.out : 0u;
+
+    // factors and terms of this thread's tokens
+    V a[R], bv[R];
+    {
+      V x[R], y[R], z[R];
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        unpack(raw[0][j], x[j], T());
+        unpack(raw[1][j], y[j], T());
+        if (P) unpack(raw[NIN - 1][j], z[j], T());
+        if (PACKED && ((m.out >> j) & 1u)) x[j] = y[j] = z[j] = V{};  // what lies outside the sequences is not used
+      }
+      if constexpr (P != 0) {
+        gates_fwd(x, y, z, cu, a, bv);
+      } else {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          a[j] = x[j];
+          bv[j] = y[j];
+        }
+      }
+    }
+    if (round + 1 < g.rounds) {
+#pragma unroll
+      for (int i = 0; i < NIN; ++i) {
+        in[i] += (long long)(cl * S::TT) * g.st[i];
+        fetch_run<true, T, VEC, R>(raw[i], in[i], g.st[i], g.T - t0 - cl * S::TT);
+      }
+    }
+    if (t0 + R > g.T) {  // behind the end the state stays
 #pragma unroll
       for (int j = 0; j < R; ++j)
-        raw[i][j] = load_raw<T, VEC>(g.in[i], b * g.sb[i] + (long long)(t0 + j) * g.st[i] + ch,
-                                     chok && t0 + j < g.T);
-    Marks m;
-    if (PACKED) m = marks_of<R>(g.starts, g.S, t0, g.T);
-    const unsigned cuts = PACKED ? m.first | m.out : 0u;
-    if (!g.fold_only && g.bounds && ty == 0 && chok && tile > 0)
-      store(g.bounds + (b * g.tiles + tile) * g.H + ch, carry);
+        if (t0 + j >= g.T) {
+          a[j] = all_of<V>(1.f);
+          bv[j] = V{};
+        }
+    }
+    if (PACKED && cuts) {
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        if (t0 + j >= g.T) continue;
+        if ((m.out >> j) & 1u) bv[j] = V{};
+        else if (((m.first >> j) & 1u) && g.h0)
+          bv[j] = vfma(a[j], m.first & ((1u << j) - 1)
+                                 ? load_f32<V>(g.h0 + (long long)seq_of(g.starts, g.S, t0 + j) * g.H + cr) : hz, bv[j]);
+      }
+    }
+    Marks next;
+    if (PACKED && round + 1 < g.rounds) {
+      next = walk.template marks<R, S::TT>(t0 + cl * S::TT - ty * R, t0 + cl * S::TT);
+      if (next.first && g.h0) hz = load_f32<V>(g.h0 + (long long)next.nf * g.H + cr);
+    }
 
-    float a[R][VEC], bv[R][VEC], A[VEC], B[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; }
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-      float x[VEC], y[VEC], z[VEC];
-      unpack(raw[0][j], x, T());
-      unpack(raw[1][j], y, T());
-      if (P) unpack(raw[NIN - 1][j], z, T());
-      if (PACKED && ((m.out >> j) & 1u)) {  // whatever lies between and behind the sequences is not used
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) x[v] = y[v] = z[v] = 0.f;
-      }
-      const bool live = t0 + j < g.T;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        if (P) {
-          const Gate q = gate_of<T>(y[v], z[v], cs[v]);
-          a[j][v] = q.a;
-          bv[j][v] = q.beta * q.sg * x[v];
-        } else {
-          a[j][v] = x[v];
-          bv[j][v] = y[v];
-        }
-        if (!live) { a[j][v] = 1.f; bv[j][v] = 0.f; }
-      }
-      if (PACKED && live) {
-        if ((m.out >> j) & 1u) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) bv[j][v] = 0.f;
-        } else if (((m.first >> j) & 1u) && g.h0 && chok) {
-          float s[VEC];
-          load_f32(g.h0 + (long long)seq_of(g.starts, g.S, t0 + j) * g.H + ch, s);
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) bv[j][v] = fmaf(a[j][v], s[v], bv[j][v]);
-        }
-      }
-      const bool cut = (cuts >> j) & 1u;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        B[v] = flow<PACKED>(cut, a[j][v], B[v], bv[j][v]);
-        A[v] *= a[j][v];
+    // fold of this thread's tokens, over the warp, over the block
+    V A, B, Ax = all_of<V>(1.f), Bx{};
+    int F = cuts != 0, Fx = 0;  // a run with a cut is the constant B
+    fold_run<PACKED>(cuts, a, bv, A, B);
+    if (S::GPW > 1) {
+      const V pa = vxor(A, LX % 32), pb = vxor(B, LX % 32);
+      const int pf = PACKED ? __shfl_xor_sync(0xffffffffu, F, LX % 32) : 0;
+      if (grp > 0) {
+        Ax = pa;
+        Bx = pb;
+        Fx = pf;
+        B = flow<PACKED>(F, A, pb, B);
+        A = vmul(A, pa);
+        F |= pf;
       }
     }
-    int F = cuts != 0;  // the run holds a cut: its A counts for nothing
+    V h;
+    if (NW > 1) {
+      const int buf = round & 1;  // the next round's barrier separates the reads from the writes after it
+      if (grp == S::GPW - 1) {
+        store(&sh.w[buf][wt][0][lx * VEC], A);
+        store(&sh.w[buf][wt][1][lx * VEC], B);
+        if (PACKED && lx == 0) sh.wf[buf][wt] = F;
+      }
+      exchange<PACKED, false>(sh, buf, cl, it.rank);
+      h = carry;
+      if (cl > 1) {
+        for (int r = 0; r < cl; ++r) {
+          if (r == it.rank) h = carry;
+          carry = flow<PACKED>(PACKED && sh.xf[buf][r] != 0, load_f32<V>(&sh.x[buf][r][0][lx * VEC]), carry,
+                               load_f32<V>(&sh.x[buf][r][1][lx * VEC]));
+        }
+      }
+      V run = h;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        if (w == wt) h = run;
+        run = flow<PACKED>(PACKED && sh.wf[buf][w] != 0, load_f32<V>(&sh.w[buf][w][0][lx * VEC]), run,
+                           load_f32<V>(&sh.w[buf][w][1][lx * VEC]));
+      }
+      if (cl == 1) carry = run;
+    } else {
+      const int src = (S::GPW - 1) * LX + lx;
+      h = carry;
+      carry = vfma(vmap(A, [&](float v) { return __shfl_sync(0xffffffffu, v, src); }), carry,
+                   vmap(B, [&](float v) { return __shfl_sync(0xffffffffu, v, src); }));
+    }
+    h = flow<PACKED>(Fx, Ax, h, Bx);
+    if (g.bounds && t0 > 0 && t0 % kScanBound == 0 && t0 < g.T && chok)
+      store(g.bounds + (b * g.nbounds + t0 / kScanBound - 1) * g.H + ch, h);
 
-    // inclusive fold over the warp's time groups, then this thread's exclusive one
-    float Ax[VEC], Bx[VEC];
+    const int left = chok ? g.T - t0 : 0;
+    if (PACKED && cuts) {
 #pragma unroll
-    for (int d = 1; d < G::GPW; d *= 2) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float pa = __shfl_up_sync(0xffffffffu, A[v], d * LX);
-        const float pb = __shfl_up_sync(0xffffffffu, B[v], d * LX);
-        if (grp >= d) {
-          B[v] = flow<PACKED>(F, A[v], pb, B[v]);
-          A[v] *= pa;
-        }
-      }
-      if (PACKED) {
-        const int pf = __shfl_up_sync(0xffffffffu, F, d * LX);
-        if (grp >= d) F |= pf;
-      }
-    }
-    const int Fx = PACKED && G::GPW > 1 ? __shfl_up_sync(0xffffffffu, F, LX % 32) : 0;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      Ax[v] = G::GPW > 1 ? __shfl_up_sync(0xffffffffu, A[v], LX % 32) : 1.f;
-      Bx[v] = G::GPW > 1 ? __shfl_up_sync(0xffffffffu, B[v], LX % 32) : 0.f;
-      if (grp == 0) { Ax[v] = 1.f; Bx[v] = 0.f; }
-    }
-    float h[VEC];
-    if (G::NW > 1) {
-      const int buf = tile & 1;  // the barrier of the next tile separates the reads from the next writes
-      if (grp == G::GPW - 1) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          sA[buf][wt][lx * VEC + v] = A[v];
-          sB[buf][wt][lx * VEC + v] = B[v];
-        }
-        if (PACKED && lx == 0) sF[buf][wt] = F;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < G::NW; ++w) {
-        const bool cut = PACKED && sF[buf][w] != 0;
-        cut_all = cut_all || cut;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          if (w == wt) h[v] = carry[v];
-          const float wa = sA[buf][w][lx * VEC + v];
-          carry[v] = flow<PACKED>(cut, wa, carry[v], sB[buf][w][lx * VEC + v]);
-          prod[v] *= wa;
-        }
+      for (int j = 0; j < R; ++j) {
+        h = flow<true>((cuts >> j) & 1u, a[j], h, bv[j]);
+        a[j] = h;
       }
     } else {
-      const int src = (lane & ~31) | ((G::GPW - 1) * LX + lx);
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float wa = __shfl_sync(0xffffffffu, A[v], src);
-        const float wb = __shfl_sync(0xffffffffu, B[v], src);
-        h[v] = carry[v];
-        carry[v] = fmaf(wa, carry[v], wb);
-        prod[v] *= wa;
+      for (int j = 0; j < R; ++j) {
+        h = vfma(a[j], h, bv[j]);
+        a[j] = h;
       }
     }
-    if (g.fold_only) continue;
-
+    if (left >= R) {
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) h[v] = flow<PACKED>(Fx && grp > 0, Ax[v], h[v], Bx[v]);
+      for (int j = 0; j < R; ++j) store(at<T>(out, j, row), a[j]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const bool cut = (cuts >> j) & 1u;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) h[v] = flow<PACKED>(cut, a[j][v], h[v], bv[j][v]);
-      const int t = t0 + j;
-      if (chok && t < g.T) {
-        store(static_cast<T*>(g.h) + (b * g.T + t) * g.H + ch, h);
-        if (PACKED && ((m.last >> j) & 1u))
-          store(g.hT + (long long)seq_of(g.starts, g.S, t) * g.H + ch, h);
-      }
+      for (int j = 0; j < R; ++j)
+        if (j < left) store(at<T>(out, j, row), a[j]);
     }
+    out += (long long)(cl * S::TT) * row;
+    if (PACKED && m.last && chok) {
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        if ((m.last >> j) & 1u)
+          store(g.hT + (long long)seq_at(m.last, m.nl, j, g.starts, g.S, t0) * g.H + ch, a[j]);
+    }
+    m = next;
   }
 
-  if (!chok) return;
-  if (PACKED && !g.fold_only && seg == 0) {  // sequences without a token pass their first state on
-    for (int n = ty; n < g.S; n += TY) {
-      if (__ldg(g.starts + n) < __ldg(g.starts + n + 1)) continue;
-      float s[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) s[v] = 0.f;
-      if (g.h0) load_f32(g.h0 + (long long)n * g.H + ch, s);
-      store(g.hT + (long long)n * g.H + ch, s);
-    }
+  if (!chok || it.rank != 0) return;
+  if (!PACKED) {
+    if (ty == 0) store(g.hT + b * g.H + ch, carry);
+    return;
   }
-  if (ty != 0) return;
-  if (g.fold_only) {
-    float* ag = g.agg + ((b * g.nseg + seg) * 2) * (long long)g.H + ch;
-    store(ag, prod);
-    store(ag + g.H, carry);
-    if (PACKED) g.seg_cut[seg] = cut_all;  // the same from every block of channels
-  } else if (!PACKED) {
-    if (tile1 == g.tiles) store(g.hT + b * g.H + ch, carry);
-  }
+  for (int n = ty; n < g.S; n += S::TY)  // sequences without a token pass their first state on
+    if (__ldg(g.starts + n) >= __ldg(g.starts + n + 1))
+      store(g.hT + (long long)n * g.H + ch, g.h0 ? load_f32<V>(g.h0 + (long long)n * g.H + ch) : V{});
+}
+
+// blocks that an SM's registers have to hold; more spill (bf16 gated: 5 against 4 blocks 184 and 205 us at
+// 8 x 2048 x 2560, the second a partial wave of blocks; fp32 spills at 5: 242 against 195 us at 1 x 32771 x 512)
+template <int P, typename T, typename S, bool PACKED>
+constexpr int bwd_blocks() {
+  if (!P) return PACKED || S::R * S::VEC > 8 ? 4 : 5;
+  if (S::R * S::VEC > 8 || sizeof(T) == 4) return 3;
+  return PACKED ? 4 : 5;
 }
 
 // ---- backward ----------------------------------------------------------------------
-template <int P, typename T, int VEC, int LX, int TY, int R, int BB, bool PACKED>
-__global__ void __launch_bounds__(kThreads) scan_bwd_kernel(ScanArgs g) {
-  using G = Geo<LX, TY>;
-  static_assert(LX * TY * BB == kThreads, "block shape");
-  static_assert(BB == 1 || G::NW == 1, "several items per block only without block barriers");
-  static_assert(!PACKED || G::NW > 1, "the one-warp tiles do not look at cuts");
-  constexpr int NIN = P ? 3 : 2;
-  constexpr int TT = TY * R;
-  __shared__ float sA[2][G::NW][LX * VEC], sB[2][G::NW][LX * VEC], sC[2][G::NW][LX * VEC];
-  __shared__ int sF[2][G::NW];
-  const int lane = threadIdx.x & 31;
-  const int lx = threadIdx.x % LX, ty = (threadIdx.x / LX) % TY;
-  const int grp = ty % G::GPW, wt = ty / G::GPW;
-  const long long item = (long long)blockIdx.x * BB + threadIdx.x / (LX * TY);
-  if (BB > 1 && item >= g.items) return;
-  const int cb = (int)(item % g.chb);
-  const long long rest = item / g.chb;
-  // the folding launch has no use for the first segment
-  const int seg = (int)(rest % g.launch_segs) + (g.fold_only ? 1 : 0);
-  const long long b = rest / g.launch_segs;
-  const int ch = cb * LX * VEC + lx * VEC;
-  const bool chok = ch < g.H;
-  const int tile0 = seg * g.seg_tiles, tile1 = min(tile0 + g.seg_tiles, g.tiles);
+template <int P, typename T, typename S, bool PACKED>
+__global__ void __launch_bounds__(S::THREADS, (bwd_blocks<P, T, S, PACKED>())) scan_bwd_kernel(ScanArgs g) {
+  static_assert(!PACKED || S::NW > 1, "the one-warp tiles do not look at cuts");
+  static_assert(S::NW == 1 || S::TT == kScanBound, "a tile starts at a saved state");
+  constexpr int NIN = P ? 3 : 2, VEC = S::VEC, R = S::R, NW = S::NW, LX = S::LX;
+  using V = typename Chans<VEC>::type;
+  __shared__ Exchange<NW, 3> sh;
+  // what only the last step of a tile needs waits in shared memory, every thread in its own places, so that
+  // five blocks fit an SM's registers instead of three
+  __shared__ V parked[P ? 4 : 1][P ? R : 1][S::THREADS];
+  const int lx = threadIdx.x % LX, ty = (threadIdx.x / LX) % S::TY;
+  const int grp = ty % S::GPW, wt = ty / S::GPW;
+  bool out_of_items;
+  const Item it = item_of<S>(g, out_of_items);
+  if (out_of_items) return;
+  const long long b = it.b;
+  const int ch = it.ch, cl = S::BB > 1 ? 1 : g.cl;
+  const bool chok = it.chok;
+  const int cr = chok ? ch : 0;
 
-  // decay gradient so far, and what its additions rounded away (a tile at a time)
-  float cs[VEC], acc[VEC], lost[VEC];
+  // carry: c behind the round; acc: decay gradient so far, lost: what its additions rounded away
+  V cu{}, carry{}, acc{}, lost{};
+  if (P) cu = vmap(load_f32<V>(g.decay + cr), [&](float d) { return rate_of(d, g.scale); });
+  const V cn = vmul(cu, all_of<V>(-0.6931471805599453f));
+  if (!PACKED && g.dhT) carry = load_f32<V>(g.dhT + b * g.H + cr);
+
+  if (cl > 1) cg::this_cluster().sync();
+  int t0 = ((g.rounds - 1) * cl + it.rank) * S::TT + ty * R;
+  const char* in[NIN + 1];
+  typename Raw<T, VEC>::type raw[NIN + 1][R];
+  V hs;  // state before the tile
+  auto first_state = [&](int tile_t0) {
+    V v{};
+    if (NW > 1 && tile_t0 > 0) {
+      if (tile_t0 < g.T) v = load_f32<V>(g.bounds + (b * g.nbounds + tile_t0 / kScanBound - 1) * g.H + cr);
+    } else if (!PACKED && g.h0) {
+      v = load_f32<V>(g.h0 + b * g.H + cr);
+    }
+    return v;
+  };
 #pragma unroll
-  for (int v = 0; v < VEC; ++v) cs[v] = acc[v] = lost[v] = 0.f;
-  if (P && chok) {
-    load_f32(g.decay + ch, cs);
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) cs[v] = -g.scale * softplus_of(cs[v]);
+  for (int i = 0; i <= NIN; ++i) {
+    const int st = g.st[i < NIN ? i : 3];
+    in[i] = reinterpret_cast<const char*>(static_cast<const T*>(i < NIN ? g.in[i < NIN ? i : 0] : g.dh) +
+                                          b * g.sb[i < NIN ? i : 3] + cr) + (long long)t0 * st;
+    fetch_run<false, T, VEC, R>(raw[i], in[i], st, i < NIN || g.dh ? g.T - t0 : 0);
   }
+  const int row = g.H * (int)sizeof(T);
+  char* out[NIN];
+#pragma unroll
+  for (int i = 0; i < NIN; ++i)
+    out[i] = reinterpret_cast<char*>(static_cast<T*>(g.d[i]) + (b * g.T + t0) * g.H + ch);
+  hs = first_state(t0 - ty * R);
 
-  // c behind the segment
-  float carry[VEC], prod[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) { carry[v] = 0.f; prod[v] = 1.f; }
-  if (!g.fold_only && chok) {
-    if (!PACKED && g.dhT) load_f32(g.dhT + b * g.H + ch, carry);
-    for (int s = g.nseg - 1; s > seg; --s) {
-      const float* ag = g.agg + ((b * g.nseg + s) * 2) * (long long)g.H + ch;
-      float fa[VEC], fb[VEC];
-      load_f32(ag, fa);
-      load_f32(ag + g.H, fb);
-      const bool cut = PACKED && g.seg_cut[s] != 0;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) carry[v] = flow<PACKED>(cut, fa[v], carry[v], fb[v]);
-    }
-  }
-  bool cut_all = false;
-
-  for (int tile = tile1 - 1; tile >= tile0; --tile) {
-    const int t0 = tile * TT + ty * R;
-    typename Raw<T, VEC>::type raw[NIN][R], rg[R];
-#pragma unroll
-    for (int i = 0; i < NIN; ++i) {
-      // a folding launch needs the decay and the incoming gradient alone
-      const bool need = !g.fold_only || (P ? i == 1 : i == 0);
-#pragma unroll
-      for (int j = 0; j < R; ++j)
-        raw[i][j] = load_raw<T, VEC>(g.in[i], b * g.sb[i] + (long long)(t0 + j) * g.st[i] + ch,
-                                     need && chok && t0 + j < g.T);
-    }
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-      rg[j] = load_raw<T, VEC>(g.dh, b * g.sb[3] + (long long)(t0 + j) * g.st[3] + ch,
-                               g.dh && chok && t0 + j < g.T);
-    float h[VEC];  // state before the tile
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) h[v] = 0.f;
-    if (!g.fold_only && chok) {
-      if (tile > 0) load_f32(g.bounds + (b * g.tiles + tile) * g.H + ch, h);
-      else if (!PACKED && g.h0) load_f32(g.h0 + b * g.H + ch, h);
-    }
-    Marks m;
-    if (PACKED) m = marks_of<R>(g.starts, g.S, t0, g.T);
+  typename WalkOf<PACKED>::type walk(g.starts, g.S, g.T);
+  Marks m = walk.template marks<R, S::TT>(t0 - ty * R, t0);
+  V hz{}, dz{};  // first state and final state's gradient that the tile needs
+  if (PACKED && m.first && g.h0) hz = load_f32<V>(g.h0 + (long long)m.nf * g.H + cr);
+  if (PACKED && m.last && g.dhT) dz = load_f32<V>(g.dhT + (long long)m.nl * g.H + cr);
+  for (int round = g.rounds - 1; round >= 0; --round, t0 -= cl * S::TT) {
     const unsigned cuts = PACKED ? m.first | m.out : 0u;
 
-    // gates; forward fold (A, B) and reverse fold (A, C) of this thread's tokens
-    float a[R][VEC], hp[R][VEC], sr[P ? R : 1][VEC], sg[P ? R : 1][VEC], be[P ? R : 1][VEC];
-    float A[VEC], B[VEC], C[VEC];
+    // gates; hp holds b_t until the states are known
+    V a[R], hp[R], gr[R], h = hs;
+    {
+      V x[R], y[R], z[R];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; C[v] = 0.f; }
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-      float x[VEC], y[VEC], z[VEC];
-      unpack(raw[0][j], x, T());
-      unpack(raw[1][j], y, T());
-      if (P) unpack(raw[NIN - 1][j], z, T());
-      if (PACKED && ((m.out >> j) & 1u)) {  // whatever lies between and behind the sequences is not used
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) x[v] = y[v] = z[v] = 0.f;
+      for (int j = 0; j < R; ++j) {
+        unpack(raw[0][j], x[j], T());
+        unpack(raw[1][j], y[j], T());
+        if (P) unpack(raw[NIN - 1][j], z[j], T());
+        unpack(raw[NIN][j], gr[j], T());
+        if (PACKED && ((m.out >> j) & 1u)) x[j] = y[j] = z[j] = gr[j] = V{};
       }
-      const bool live = t0 + j < g.T;
+      if constexpr (P != 0) {
+        V s[R], w[R], k[R], mg[R];
+        gates_bwd(x, y, z, cu, a, w, s, hp, k, mg);
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        if (P) {
-          const Gate q = gate_of<T>(y[v], z[v], cs[v]);
-          a[j][v] = q.a;
-          hp[j][v] = q.beta * q.sg * x[v];  // b_t, replaced below by the state before t
-          sr[j][v] = q.sr;
-          sg[j][v] = q.sg;
-          be[j][v] = q.beta;
-        } else {
-          a[j][v] = x[v];
-          hp[j][v] = y[v];
+        for (int j = 0; j < R; ++j) {
+          parked[0][j][threadIdx.x] = s[j];
+          parked[1][j][threadIdx.x] = w[j];
+          parked[2][j][threadIdx.x] = k[j];
+          parked[3][j][threadIdx.x] = mg[j];
         }
-        if (!live) { a[j][v] = 1.f; hp[j][v] = 0.f; }
-      }
-      if (PACKED && live) {
-        if ((m.out >> j) & 1u) {
+      } else {
 #pragma unroll
-          for (int v = 0; v < VEC; ++v) hp[j][v] = 0.f;
-        } else if (((m.first >> j) & 1u) && g.h0 && chok) {
-          float s[VEC];
-          load_f32(g.h0 + (long long)seq_of(g.starts, g.S, t0 + j) * g.H + ch, s);
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) hp[j][v] = fmaf(a[j][v], s[v], hp[j][v]);
+        for (int j = 0; j < R; ++j) {
+          a[j] = x[j];
+          hp[j] = y[j];
         }
-      }
-      const bool cut = (cuts >> j) & 1u;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        B[v] = flow<PACKED>(cut, a[j][v], B[v], hp[j][v]);
-        A[v] *= a[j][v];
       }
     }
-    float gr[R][VEC];
+    if (round > 0) {
 #pragma unroll
-    for (int j = R - 1; j >= 0; --j) {
-      unpack(rg[j], gr[j], T());
-      if (PACKED) {
-        if ((m.out >> j) & 1u) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) gr[j][v] = 0.f;
-        } else if (((m.last >> j) & 1u) && g.dhT && chok) {
-          float s[VEC];
-          load_f32(g.dhT + (long long)seq_of(g.starts, g.S, t0 + j) * g.H + ch, s);
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) gr[j][v] += s[v];
-        }
+      for (int i = 0; i <= NIN; ++i) {
+        const int st = g.st[i < NIN ? i : 3];
+        in[i] -= (long long)(cl * S::TT) * st;
+        fetch_run<false, T, VEC, R>(raw[i], in[i], st, i < NIN || g.dh ? g.T - t0 + cl * S::TT : 0);
       }
+      hs = first_state(t0 - cl * S::TT - ty * R);
+    }
+    if (t0 + R > g.T) {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) C[v] = PACKED && ((cuts >> j) & 1u) ? 0.f : a[j][v] * (gr[j][v] + C[v]);
+      for (int j = 0; j < R; ++j)
+        if (t0 + j >= g.T) {
+          a[j] = all_of<V>(1.f);
+          hp[j] = V{};
+        }
+    }
+    if (PACKED && (cuts | m.last)) {
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        if (t0 + j >= g.T) continue;
+        if ((m.out >> j) & 1u) hp[j] = V{};
+        if (((m.first >> j) & 1u) && g.h0)
+          hp[j] = vfma(a[j], m.first & ((1u << j) - 1)
+                                 ? load_f32<V>(g.h0 + (long long)seq_of(g.starts, g.S, t0 + j) * g.H + cr) : hz, hp[j]);
+        if (((m.last >> j) & 1u) && g.dhT)
+          gr[j] = vadd(gr[j], m.last & ((1u << j) - 1)
+                                  ? load_f32<V>(g.dhT + (long long)seq_of(g.starts, g.S, t0 + j) * g.H + cr) : dz);
+      }
+    }
+    const V h0f = hz;
+    Marks next;
+    if (PACKED && round > 0) {
+      next = walk.template marks<R, S::TT>(t0 - cl * S::TT - ty * R, t0 - cl * S::TT);
+      if (next.first && g.h0) hz = load_f32<V>(g.h0 + (long long)next.nf * g.H + cr);
+      if (next.last && g.dhT) dz = load_f32<V>(g.dhT + (long long)next.nl * g.H + cr);
     }
 
-    // folds over the warp's time groups: forward from the left, reverse from the right
-    float Ax[VEC], Bx[VEC], Ar[VEC], Cx[VEC], At[VEC], Bt[VEC], Ct[VEC];
+    // forward fold (A, B) and reverse fold (A, C) of this thread's tokens
+    V A, B, C{};
+    const int F = cuts != 0;
+    fold_run<PACKED>(cuts, a, hp, A, B);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) Ar[v] = A[v];
-    int F = cuts != 0, Fr = F;
-#pragma unroll
-    for (int d = 1; d < G::GPW; d *= 2) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float pa = __shfl_up_sync(0xffffffffu, A[v], d * LX);
-        const float pb = __shfl_up_sync(0xffffffffu, B[v], d * LX);
-        const float na = __shfl_down_sync(0xffffffffu, Ar[v], d * LX);
-        const float nc = __shfl_down_sync(0xffffffffu, C[v], d * LX);
-        if (grp >= d) {
-          B[v] = flow<PACKED>(F, A[v], pb, B[v]);
-          A[v] *= pa;
-        }
-        if (grp + d < G::GPW) {
-          C[v] = flow<PACKED>(Fr, Ar[v], nc, C[v]);
-          Ar[v] *= na;
-        }
-      }
-      if (PACKED) {
-        const int pf = __shfl_up_sync(0xffffffffu, F, d * LX);
-        const int nf = __shfl_down_sync(0xffffffffu, Fr, d * LX);
-        if (grp >= d) F |= pf;
-        if (grp + d < G::GPW) Fr |= nf;
-      }
-    }
-    const int hi_lane = (G::GPW - 1) * LX + lx;
-    const int Fx = PACKED && G::GPW > 1 ? __shfl_up_sync(0xffffffffu, F, LX % 32) : 0;
-    const int Fy = PACKED && G::GPW > 1 ? __shfl_down_sync(0xffffffffu, Fr, LX % 32) : 0;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      // the warp's whole fold: forward at its last group, reverse at its first
-      At[v] = __shfl_sync(0xffffffffu, A[v], hi_lane);
-      Bt[v] = __shfl_sync(0xffffffffu, B[v], hi_lane);
-      Ct[v] = __shfl_sync(0xffffffffu, C[v], lx);
-      Ax[v] = G::GPW > 1 ? __shfl_up_sync(0xffffffffu, A[v], LX % 32) : 1.f;
-      Bx[v] = G::GPW > 1 ? __shfl_up_sync(0xffffffffu, B[v], LX % 32) : 0.f;
-      Ar[v] = G::GPW > 1 ? __shfl_down_sync(0xffffffffu, Ar[v], LX % 32) : 1.f;
-      Cx[v] = G::GPW > 1 ? __shfl_down_sync(0xffffffffu, C[v], LX % 32) : 0.f;
-      if (grp == 0) { Ax[v] = 1.f; Bx[v] = 0.f; }
-      if (grp == G::GPW - 1) { Ar[v] = 1.f; Cx[v] = 0.f; }
-    }
-    float c[VEC];
-    if (G::NW > 1) {
-      const int buf = tile & 1;
+    for (int j = R - 1; j >= 0; --j) C = PACKED && ((cuts >> j) & 1u) ? V{} : vmul(a[j], vadd(gr[j], C));
+    // the two groups of a warp: the first one's fold goes to the second's states, the second one's to the
+    // first's adjoints, and both make the warp's
+    V Ax = all_of<V>(1.f), Bx{}, Cx{}, At = A, Bt = B, Ct = C;
+    int Fo = 0;
+    if (S::GPW > 1) {
+      if (PACKED) Fo = __shfl_xor_sync(0xffffffffu, F, LX % 32);
+      Ax = vxor(A, LX % 32);
+      Bx = vxor(B, LX % 32);
+      Cx = vxor(C, LX % 32);
+      At = vmul(A, Ax);
       if (grp == 0) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          sA[buf][wt][lx * VEC + v] = At[v];
-          sB[buf][wt][lx * VEC + v] = Bt[v];
-          sC[buf][wt][lx * VEC + v] = Ct[v];
-        }
-        if (PACKED && lx == 0) sF[buf][wt] = Fr;  // the first group's: the whole warp's
-      }
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < G::NW; ++w) {
-        const bool cut = PACKED && sF[buf][w] != 0;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-          if (w < wt) h[v] = flow<PACKED>(cut, sA[buf][w][lx * VEC + v], h[v], sB[buf][w][lx * VEC + v]);
-      }
-#pragma unroll
-      for (int w = G::NW - 1; w >= 0; --w) {
-        const bool cut = PACKED && sF[buf][w] != 0;
-        cut_all = cut_all || cut;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          if (w == wt) c[v] = carry[v];
-          const float wa = sA[buf][w][lx * VEC + v];
-          carry[v] = flow<PACKED>(cut, wa, carry[v], sC[buf][w][lx * VEC + v]);
-          prod[v] *= wa;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        c[v] = carry[v];
-        carry[v] = fmaf(At[v], carry[v], Ct[v]);
-        prod[v] *= At[v];
+        Bt = flow<PACKED>(Fo, Ax, B, Bx);
+        Ct = flow<PACKED>(F, A, Cx, C);
+      } else {
+        Bt = flow<PACKED>(F, A, Bx, B);
+        Ct = flow<PACKED>(Fo, Ax, C, Cx);
       }
     }
-    if (g.fold_only) continue;
+    V c;
+    if (NW > 1) {
+      const int buf = round & 1;
+      if (grp == 0) {
+        store(&sh.w[buf][wt][0][lx * VEC], At);
+        store(&sh.w[buf][wt][1][lx * VEC], Bt);
+        store(&sh.w[buf][wt][2][lx * VEC], Ct);
+        if (PACKED && lx == 0) sh.wf[buf][wt] = F | Fo;
+      }
+      exchange<PACKED, true>(sh, buf, cl, it.rank);
+      c = carry;
+      if (cl > 1) {
+        for (int r = cl - 1; r >= 0; --r) {
+          if (r == it.rank) c = carry;
+          carry = flow<PACKED>(PACKED && sh.xf[buf][r] != 0, load_f32<V>(&sh.x[buf][r][0][lx * VEC]), carry,
+                               load_f32<V>(&sh.x[buf][r][1][lx * VEC]));
+        }
+      }
+      V run = c;
+#pragma unroll
+      for (int u = NW - 1; u >= 0; --u) {
+        const bool cut = PACKED && sh.wf[buf][u] != 0;
+        const V wa = load_f32<V>(&sh.w[buf][u][0][lx * VEC]);
+        if (u == wt) c = run;
+        run = flow<PACKED>(cut, wa, run, load_f32<V>(&sh.w[buf][u][2][lx * VEC]));
+      }
+      if (cl == 1) carry = run;
+#pragma unroll
+      for (int u = 0; u < NW - 1; ++u)
+        if (u < wt)
+          h = flow<PACKED>(PACKED && sh.wf[buf][u] != 0, load_f32<V>(&sh.w[buf][u][0][lx * VEC]), h,
+                           load_f32<V>(&sh.w[buf][u][1][lx * VEC]));
+    } else {
+      c = carry;
+      carry = vfma(At, carry, Ct);
+    }
+    if (S::GPW > 1) {
+      if (grp > 0) h = flow<PACKED>(Fo, Ax, h, Bx);
+      else c = flow<PACKED>(Fo, Ax, c, Cx);
+    }
 
     // states before each token, then the adjoint from the last token to the first
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      h[v] = flow<PACKED>(Fx && grp > 0, Ax[v], h[v], Bx[v]);
-      c[v] = flow<PACKED>(Fy && grp < G::GPW - 1, Ar[v], c[v], Cx[v]);
-    }
-#pragma unroll
     for (int j = 0; j < R; ++j) {
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float nx = flow<PACKED>((cuts >> j) & 1u, a[j][v], h[v], hp[j][v]);
-        hp[j][v] = h[v];
-        h[v] = nx;
-      }
+      const V nx = flow<PACKED>((cuts >> j) & 1u, a[j], h, hp[j]);
+      hp[j] = h;
+      h = nx;
     }
-    float tacc[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) tacc[v] = 0.f;
+    V tacc{};
+    const int left = chok ? g.T - t0 : 0;
+    const bool whole = left >= R;
 #pragma unroll
     for (int j = R - 1; j >= 0; --j) {
-      const int t = t0 + j;
-      const bool live = chok && t < g.T;
-      float lam[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        lam[v] = gr[j][v] + c[v];
-        c[v] = PACKED && ((cuts >> j) & 1u) ? 0.f : a[j][v] * lam[v];
-      }
-      if (PACKED) {
+      V lam = vadd(gr[j], c);
+      c = PACKED && ((cuts >> j) & 1u) ? V{} : vmul(a[j], lam);
+      if (PACKED && ((cuts >> j) & 1u)) {
+        hp[j] = V{};
         if ((m.out >> j) & 1u) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) lam[v] = hp[j][v] = 0.f;
-        } else if ((m.first >> j) & 1u) {
-          const long long n = seq_of(g.starts, g.S, t);
-          float s[VEC];
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) hp[j][v] = 0.f;
-          if (g.h0 && chok) load_f32(g.h0 + n * g.H + ch, hp[j]);
-          if (g.dh0 && live) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) s[v] = a[j][v] * lam[v];
-            store(g.dh0 + n * g.H + ch, s);
-          }
+          lam = V{};
+        } else if (j < left) {
+          const long long n = seq_at(m.first, m.nf, j, g.starts, g.S, t0);
+          if (g.h0) hp[j] = m.first & ((1u << j) - 1) ? load_f32<V>(g.h0 + n * g.H + cr) : h0f;
+          if (g.dh0) store(g.dh0 + n * g.H + ch, vmul(a[j], lam));
         }
       }
-      if (!live) continue;
-      const long long off = (b * g.T + t) * g.H + ch;
-      if (P) {
-        float x[VEC], d0[VEC], d1[VEC], d2[VEC];
-        unpack(raw[0][j], x, T());
-        if (PACKED && ((m.out >> j) & 1u)) {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) x[v] = 0.f;
+      const bool live = whole || j < left;
+      if constexpr (P != 0) {
+        // L_t (1 - s) = -ln(2) cu s (1 - s)
+        const V s = parked[0][j][threadIdx.x];
+        const V dl = vmul(lam, vfma(hp[j], a[j], parked[2][j][threadIdx.x]));
+        const V cs = vmul(cn, s);
+        const V d1 = vmul(dl, vfma(cs, vmul(s, all_of<V>(-1.f)), cs));
+        if (live) {
+          store(at<T>(out[0], j, row), vmul(lam, parked[1][j][threadIdx.x]));
+          store(at<T>(out[1], j, row), d1);
+          store(at<T>(out[NIN - 1], j, row), vmul(lam, parked[3][j][threadIdx.x]));
+          tacc = vfma(dl, s, tacc);
         }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const float s = sr[j][v], q = sg[j][v], bt = be[j][v], av = a[j][v];
-          const float L = cs[v] * s, lb = lam[v] * bt, lq = lam[v] * q * x[v];
-          d0[v] = lb * q;
-          d2[v] = lb * x[v] * q * (1.f - q);
-          // dL/dL_t = a dL/da + dL/dbeta * (-a^2 / beta); with beta = 0 (L = 0) its share of the
-          // gradients below tends to 0
-          float dl = lam[v] * hp[j][v] * av;
-          if (bt > 0.f) dl = fmaf(-lq * av * av, rcp_approx(bt), dl);
-          d1[v] = dl * L * (1.f - s);
-          tacc[v] = fmaf(dl, s, tacc[v]);
-        }
-        store(static_cast<T*>(g.d[0]) + off, d0);
-        store(static_cast<T*>(g.d[1]) + off, d1);
-        store(static_cast<T*>(g.d[2]) + off, d2);
-      } else {
-        float d0[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) d0[v] = lam[v] * hp[j][v];
-        store(static_cast<T*>(g.d[0]) + off, d0);
-        store(static_cast<T*>(g.d[1]) + off, lam);
+      } else if (live) {
+        store(at<T>(out[0], j, row), vmul(lam, hp[j]));
+        store(at<T>(out[1], j, row), lam);
       }
     }
-    if (P) {
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {  // compensated sum
-        const float y = tacc[v] - lost[v], t = acc[v] + y;
-        lost[v] = (t - acc[v]) - y;
-        acc[v] = t;
-      }
+    for (int i = 0; i < NIN; ++i) out[i] -= (long long)(cl * S::TT) * row;
+    m = next;
+    if (P) {  // compensated sum
+      const V y = vfma(lost, all_of<V>(-1.f), tacc), t = vadd(acc, y);
+      lost = vfma(y, all_of<V>(-1.f), vfma(acc, all_of<V>(-1.f), t));
+      acc = t;
     }
   }
 
-  if (g.fold_only) {
-    if (chok && ty == 0) {
-      float* ag = g.agg + ((b * g.nseg + seg) * 2) * (long long)g.H + ch;
-      store(ag, prod);
-      store(ag + g.H, carry);
-      if (PACKED) g.seg_cut[seg] = cut_all;
-    }
-    return;
-  }
-  if (P) {  // decay gradient of this item: fixed order over the time groups
-#pragma unroll
-    for (int v = 0; v < VEC; ++v)
-#pragma unroll
-      for (int d = LX; d < 32; d *= 2) acc[v] += __shfl_xor_sync(0xffffffffu, acc[v], d);
-    if (G::NW > 1) {
+  if (P) {  // decay gradient of this block or warp: fixed order over the time groups
+    if (S::GPW > 1) acc = vadd(acc, vxor(acc, LX % 32));
+    if (NW > 1) {
       __syncthreads();
-      if (grp == 0) {
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) sA[0][wt][lx * VEC + v] = acc[v];
-      }
+      if (grp == 0) store(&sh.w[0][wt][0][lx * VEC], acc);
       __syncthreads();
+      acc = V{};
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        acc[v] = 0.f;
-#pragma unroll
-        for (int w = 0; w < G::NW; ++w) acc[v] += sA[0][w][lx * VEC + v];
-      }
+      for (int u = 0; u < NW; ++u) acc = vadd(acc, load_f32<V>(&sh.w[0][u][0][lx * VEC]));
     }
-    if (chok && ty == 0) store(g.part + (b * g.nseg + seg) * g.H + ch, acc);
+    if (chok && ty == 0) store(g.part + (b * cl + it.rank) * g.H + ch, acc);
   }
-  if (!chok || seg != 0 || !g.dh0) return;
+  if (!chok || it.rank != 0 || !g.dh0) return;
   if (!PACKED) {
     if (ty == 0) store(g.dh0 + b * g.H + ch, carry);
-  } else {
-    for (int n = ty; n < g.S; n += TY) {
-      if (__ldg(g.starts + n) < __ldg(g.starts + n + 1)) continue;
-      float s[VEC];
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) s[v] = 0.f;
-      if (g.dhT) load_f32(g.dhT + (long long)n * g.H + ch, s);
-      store(g.dh0 + (long long)n * g.H + ch, s);
-    }
+    return;
   }
+  for (int n = ty; n < g.S; n += S::TY)
+    if (__ldg(g.starts + n) >= __ldg(g.starts + n + 1))
+      store(g.dh0 + (long long)n * g.H + ch, g.dhT ? load_f32<V>(g.dhT + (long long)n * g.H + ch) : V{});
 }
 
 // d loss / d decay = -scale sigmoid(decay) * sum of the items' partial sums, in fixed order
@@ -797,7 +916,7 @@ __global__ void __launch_bounds__(1024) decay_finish_kernel(const float* part, l
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   const int cc = blockIdx.x * 32 + threadIdx.y;
-  if (threadIdx.x == 0 && cc < H) out[cc] = -scale * sigmoid_of<float>(decay[cc]) * (float)v;
+  if (threadIdx.x == 0 && cc < H) out[cc] = -scale * sigmoid_of(decay[cc]) * (float)v;
 }
 
 // One token for each of B sequences: the whole call is one launch without any exchange.
@@ -808,18 +927,21 @@ __global__ void __launch_bounds__(kThreads) gated_step_kernel(ScanArgs g) {
   if (i >= (long long)g.B * hv) return;
   const long long b = i / hv;
   const int ch = (int)(i - b * hv) * VEC;
-  float x[VEC], r[VEC], q[VEC], d[VEC], s[VEC];
-  unpack(load_raw<T, VEC>(g.in[0], b * g.sb[0] + ch, true), x, T());
-  unpack(load_raw<T, VEC>(g.in[1], b * g.sb[1] + ch, true), r, T());
-  unpack(load_raw<T, VEC>(g.in[2], b * g.sb[2] + ch, true), q, T());
-  load_f32(g.decay + ch, d);
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) s[v] = 0.f;
-  if (g.h0) load_f32(g.h0 + b * g.H + ch, s);
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    const Gate k = gate_of<T>(r[v], q[v], -g.scale * softplus_of(d[v]));
-    s[v] = fmaf(k.a, s[v], k.beta * k.sg * x[v]);
+  using V = typename Chans<VEC>::type;
+  V x, r, q;
+  unpack(load_raw<T, VEC>(static_cast<const T*>(g.in[0]) + b * g.sb[0] + ch), x, T());
+  unpack(load_raw<T, VEC>(static_cast<const T*>(g.in[1]) + b * g.sb[1] + ch), r, T());
+  unpack(load_raw<T, VEC>(static_cast<const T*>(g.in[2]) + b * g.sb[2] + ch), q, T());
+  const V cu = vmap(load_f32<V>(g.decay + ch), [&](float d) { return rate_of(d, g.scale); });
+  V s = g.h0 ? load_f32<V>(g.h0 + b * g.H + ch) : V{};
+  if constexpr (VEC == 2) {
+    float2 a, w;
+    gate_fwd(r, q, cu, a, w);
+    s = fma2(a, s, mul2(w, x));
+  } else {
+    float2 a, w;
+    gate_fwd(two(r), two(q), two(cu), a, w);
+    s = fmaf(a.x, s, w.x * x);
   }
   store(g.hT + b * g.H + ch, s);  // may be the array h0 was read from: same thread, same place
   store(static_cast<T*>(g.h) + b * g.H + ch, s);
@@ -827,46 +949,86 @@ __global__ void __launch_bounds__(kThreads) gated_step_kernel(ScanArgs g) {
 
 bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-// whether every row can be read and written 4 channels at a time
-bool vec_ok(const ScanArgs& a, int nin, int esize, bool bwd) {
-  const size_t n = 4 * (size_t)esize;
-  bool ok = a.H % 4 == 0;
-  for (int i = 0; i < nin; ++i) ok = ok && aligned(a.in[i], n) && a.sb[i] % 4 == 0 && a.st[i] % 4 == 0;
+// whether every row can be read and written two channels at a time
+bool pairs_ok(const ScanArgs& a, int nin, int esize, bool bwd) {
+  const size_t n = 2 * (size_t)esize;
+  bool ok = a.H % 2 == 0;
+  for (int i = 0; i < nin; ++i) ok = ok && aligned(a.in[i], n) && a.sb[i] % 2 == 0 && a.st[i] % (int)n == 0;
   if (bwd) {
-    ok = ok && aligned(a.dh, n) && a.sb[3] % 4 == 0 && a.st[3] % 4 == 0;
+    ok = ok && aligned(a.dh, n) && a.sb[3] % 2 == 0 && a.st[3] % (int)n == 0;
     for (int i = 0; i < nin; ++i) ok = ok && aligned(a.d[i], n);
   } else {
     ok = ok && aligned(a.h, n);
   }
-  return ok && aligned(a.decay, 16) && aligned(a.h0, 16) && aligned(a.hT, 16) && aligned(a.dhT, 16) &&
-         aligned(a.dh0, 16) && aligned(a.bounds, 16) && aligned(a.agg, 16) && aligned(a.part, 16);
+  return ok && aligned(a.decay, 8) && aligned(a.h0, 8) && aligned(a.hT, 8) && aligned(a.dhT, 8) &&
+         aligned(a.dh0, 8) && aligned(a.bounds, 8) && aligned(a.part, 8);
 }
 
-template <int P, typename T, int VEC, int LX, int TY, int R, int BB, bool PACKED>
-cudaError_t launch_one(ScanArgs a, bool bwd, cudaStream_t st) {
-  a.chb = (a.H + LX * VEC - 1) / (LX * VEC);
-  for (int pass = a.nseg > 1 ? 0 : 1; pass < 2; ++pass) {
-    a.fold_only = pass == 0;
-    a.launch_segs = pass == 0 ? a.nseg - 1 : a.nseg;  // one end segment is never folded
-    a.items = (long long)a.B * a.launch_segs * a.chb;
-    const long long blocks = (a.items + BB - 1) / BB;
-    if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    if (bwd) scan_bwd_kernel<P, T, VEC, LX, TY, R, BB, PACKED><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-    else scan_fwd_kernel<P, T, VEC, LX, TY, R, BB, PACKED><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-    const cudaError_t e = cudaGetLastError();
+template <typename S, typename K>
+cudaError_t launch_one(K kernel, ScanArgs a, cudaStream_t st) {
+  a.chb = (a.H + kItem - 1) / kItem;
+  a.items = (long long)a.B * a.chb;
+  if (S::BB > 1) a.cl = 1;
+  const int tiles = (a.T + S::TT - 1) / S::TT;
+  a.rounds = (tiles + a.cl - 1) / a.cl;
+  const long long blocks = S::BB > 1 ? (a.items + S::BB - 1) / S::BB : a.items * a.cl;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(S::THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)a.cl;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.cl > 1 ? 1 : 0;
+  if (a.cl > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
   }
-  return cudaSuccess;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
 }
+
+// VEC, tokens per thread, threads along time, items per block
+using FwdPair = Shape<2, 8, 8, 1>;
+using FwdOne = Shape<1, 16, 4, 1>;
+using BwdPair = Shape<2, 4, 8, 1>;
+using BwdOne = Shape<1, 8, 4, 1>;
+using ShortPair = Shape<2, 8, 2, 4>;
+using ShortOne = Shape<1, 16, 1, 4>;
+using TinyPair = Shape<2, 4, 2, 4>;
+using TinyOne = Shape<1, 8, 1, 4>;
 
 template <int P, typename T>
 cudaError_t launch_typed(const ScanArgs& a, bool bwd, cudaStream_t st) {
-  const bool vec = vec_ok(a, P ? 3 : 2, (int)sizeof(T), bwd);
-  if (a.starts)
-    return vec ? launch_one<P, T, 4, 8, 16, 4, 1, true>(a, bwd, st) : launch_one<P, T, 1, 32, 4, 16, 1, true>(a, bwd, st);
-  if (a.tile == kScanShortTile)
-    return vec ? launch_one<P, T, 4, 8, 4, 4, 4, false>(a, bwd, st) : launch_one<P, T, 1, 32, 1, 16, 4, false>(a, bwd, st);
-  return vec ? launch_one<P, T, 4, 8, 16, 4, 1, false>(a, bwd, st) : launch_one<P, T, 1, 32, 4, 16, 1, false>(a, bwd, st);
+  const bool pair = pairs_ok(a, P ? 3 : 2, (int)sizeof(T), bwd);
+  if (a.starts) {
+    if (bwd)
+      return pair ? launch_one<BwdPair>(scan_bwd_kernel<P, T, BwdPair, true>, a, st)
+                  : launch_one<BwdOne>(scan_bwd_kernel<P, T, BwdOne, true>, a, st);
+    return pair ? launch_one<FwdPair>(scan_fwd_kernel<P, T, FwdPair, true>, a, st)
+                : launch_one<FwdOne>(scan_fwd_kernel<P, T, FwdOne, true>, a, st);
+  }
+  if (a.T <= TinyPair::TT) {
+    if (bwd)
+      return pair ? launch_one<TinyPair>(scan_bwd_kernel<P, T, TinyPair, false>, a, st)
+                  : launch_one<TinyOne>(scan_bwd_kernel<P, T, TinyOne, false>, a, st);
+    return pair ? launch_one<TinyPair>(scan_fwd_kernel<P, T, TinyPair, false>, a, st)
+                : launch_one<TinyOne>(scan_fwd_kernel<P, T, TinyOne, false>, a, st);
+  }
+  if (a.T <= kScanShort) {
+    if (bwd)
+      return pair ? launch_one<ShortPair>(scan_bwd_kernel<P, T, ShortPair, false>, a, st)
+                  : launch_one<ShortOne>(scan_bwd_kernel<P, T, ShortOne, false>, a, st);
+    return pair ? launch_one<ShortPair>(scan_fwd_kernel<P, T, ShortPair, false>, a, st)
+                : launch_one<ShortOne>(scan_fwd_kernel<P, T, ShortOne, false>, a, st);
+  }
+  if (bwd)
+    return pair ? launch_one<BwdPair>(scan_bwd_kernel<P, T, BwdPair, false>, a, st)
+                : launch_one<BwdOne>(scan_bwd_kernel<P, T, BwdOne, false>, a, st);
+  return pair ? launch_one<FwdPair>(scan_fwd_kernel<P, T, FwdPair, false>, a, st)
+              : launch_one<FwdOne>(scan_fwd_kernel<P, T, FwdOne, false>, a, st);
 }
 
 template <int P>
@@ -880,11 +1042,11 @@ cudaError_t launch_policy(const ScanArgs& a, int dtype, bool bwd, cudaStream_t s
 
 template <typename T>
 cudaError_t launch_step(const ScanArgs& a, cudaStream_t st) {
-  const bool vec = vec_ok(a, 3, (int)sizeof(T), false);
-  const long long n = (long long)a.B * (vec ? a.H / 4 : a.H);
+  const bool pair = pairs_ok(a, 3, (int)sizeof(T), false);
+  const long long n = (long long)a.B * (pair ? a.H / 2 : a.H);
   const long long blocks = (n + kThreads - 1) / kThreads;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  if (vec) gated_step_kernel<T, 4><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+  if (pair) gated_step_kernel<T, 2><<<(unsigned)blocks, kThreads, 0, st>>>(a);
   else gated_step_kernel<T, 1><<<(unsigned)blocks, kThreads, 0, st>>>(a);
   return cudaGetLastError();
 }
@@ -893,25 +1055,20 @@ cudaError_t launch_step(const ScanArgs& a, cudaStream_t st) {
 
 ScanPlan plan_scan(int B, int T, int H, bool packed, int num_sms) {
   ScanPlan p;
-  const long long groups = (H + 31) / 32;  // a block or a warp covers 32 channels in every variant
-  p.tile = !packed && T <= kScanShortTile ? kScanShortTile : kScanLongTile;
-  p.tiles = (T + p.tile - 1) / p.tile;
-  const long long chains = B * groups;
-  const long long want = 4LL * num_sms;  // blocks that fill the GPU
-  long long seg = 1;
-  if (chains < want) seg = (want + chains - 1) / chains;
-  const long long most = p.tiles / 4;  // at least 4 tiles a segment
-  if (seg > most) seg = most;
-  if (seg < 1) seg = 1;
-  p.seg_tiles = (int)((p.tiles + seg - 1) / seg);
-  p.nseg = (p.tiles + p.seg_tiles - 1) / p.seg_tiles;
+  p.nbounds = (T - 1) / kScanBound;
+  const long long items = (long long)B * ((H + kItem - 1) / kItem);
+  p.cl = 1;
+  if (packed || T > kScanShort) {
+    const int tiles = (T + kScanBound - 1) / kScanBound;
+    while (p.cl < kScanMaxCluster && items * p.cl * 2 <= 5LL * num_sms && p.cl * 4 <= tiles) p.cl *= 2;
+  }
   return p;
 }
 
 cudaError_t launch_scan(const ScanArgs& a, int policy, int dtype, bool bwd, cudaStream_t st) {
   const cudaError_t e = policy ? launch_policy<1>(a, dtype, bwd, st) : launch_policy<0>(a, dtype, bwd, st);
   if (e != cudaSuccess || !bwd || !policy) return e;
-  decay_finish_kernel<<<(a.H + 31) / 32, dim3(32, 32), 0, st>>>(a.part, (long long)a.B * a.nseg, a.H, a.decay,
+  decay_finish_kernel<<<(a.H + 31) / 32, dim3(32, 32), 0, st>>>(a.part, (long long)a.B * a.cl, a.H, a.decay,
                                                                a.scale, a.ddecay);
   return cudaGetLastError();
 }

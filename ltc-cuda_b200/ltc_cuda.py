@@ -32,6 +32,7 @@ kernels raises ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import logging
 import os
 import threading
@@ -86,7 +87,7 @@ class LtcScanInput(ctypes.Structure):
 
 class LtcScanPlan(ctypes.Structure):
     _fields_ = [("saved_bytes", ctypes.c_size_t), ("fwd_workspace_bytes", ctypes.c_size_t),
-                ("bwd_workspace_bytes", ctypes.c_size_t), ("tile", ctypes.c_int32), ("segments", ctypes.c_int32)]
+                ("bwd_workspace_bytes", ctypes.c_size_t), ("cluster", ctypes.c_int32)]
 
 
 class LtcLogits(ctypes.Structure):
@@ -679,6 +680,7 @@ def ltc_preamble(x, ln_w, ln_b, in_w, in_b, eps: float):
 # ---------------------------------------------------------------------------
 # Linear recurrences, parallel over time
 # ---------------------------------------------------------------------------
+SCAN_MAX_H = 1 << 28
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -701,7 +703,7 @@ def _on_cuda(t: torch.Tensor, name: str) -> None:
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """Channels contiguous, any strides before them."""
+    """Channels contiguous, strides before them as they are."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
@@ -713,7 +715,42 @@ def _scan_input(t: torch.Tensor) -> LtcScanInput:
 
 
 def _current_stream(dev) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+class _OnDevice:
+    """``torch.cuda.device`` for the common case that the device is the current one already."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, dev):
+        self.guard = None if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+@functools.lru_cache(maxsize=1024)
+def _scan_plan(index: int, dims: Tuple[int, int, int, int], dtype: int) -> Tuple[int, int, int]:
+    """(saved, forward workspace, backward workspace) bytes on the current device, number ``index``."""
+    p = LtcScanPlan()
+    B, T, H, S = dims
+    _check(_lib.ltc_scan_plan(ctypes.byref(LtcScanDims(B, T, H, dtype, S)), ctypes.byref(p)), "ltc_scan_plan")
+    return p.saved_bytes, p.fwd_workspace_bytes, p.bwd_workspace_bytes
+
+
+def _alike(t, name: str, first: torch.Tensor) -> None:
+    """``t`` has the type, place and shape of ``first``."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is first.dtype and t.device == first.device):
+        _typed(t, name, first.dtype, first.device)
+    if t.shape != first.shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(first.shape)}")
 
 
 def _scan_operands(names, tensors, h0, seq_starts):
@@ -724,12 +761,10 @@ def _scan_operands(names, tensors, h0, seq_starts):
         raise ValueError(f"{names[0]} must be {'(B, T, H)' if want == 3 else '(tokens, H) with seq_starts'}, "
                          f"got shape {tuple(first.shape)}")
     for t, n in zip(tensors[1:], names[1:]):
-        _typed(t, n, first.dtype, first.device)
-        if t.shape != first.shape:
-            raise ValueError(f"{n} has shape {tuple(t.shape)}, expected {tuple(first.shape)}")
-    H = first.shape[-1]
+        _alike(t, n, first)
     if seq_starts is None:
-        B, T, S = first.shape[0], first.shape[1], 0
+        B, T, H = first.shape
+        S = 0
     else:
         if not isinstance(seq_starts, torch.Tensor) or seq_starts.dtype not in (torch.int32, torch.int64):
             raise TypeError("seq_starts must be an int32 or int64 tensor")
@@ -737,13 +772,14 @@ def _scan_operands(names, tensors, h0, seq_starts):
             raise ValueError("seq_starts must hold S + 1 >= 2 token offsets")
         if seq_starts.device != first.device:
             raise ValueError(f"seq_starts is on {seq_starts.device}, expected {first.device}")
-        B, T, S = 1, first.shape[0], seq_starts.numel() - 1
+        T, H = first.shape
+        B, S = 1, seq_starts.numel() - 1
         seq_starts = seq_starts.to(torch.int32).contiguous()
-    if T > 0x7fffff00:
-        raise ValueError(f"{T} time steps are more than a row may have (2^31 - 256)")
+    if T > 0x7fffff00 or H > SCAN_MAX_H or any(t.stride(-2) > SCAN_MAX_H for t in tensors):
+        raise ValueError("more than 2^31 - 256 time steps, 2^28 channels, or a time stride past 2^28 elements")
     if h0 is not None:
         h0 = _as_f32(h0, first.device, "h0")
-        if tuple(h0.shape) != (S or B, H):
+        if h0.shape != (S or B, H):
             raise ValueError(f"h0 has shape {tuple(h0.shape)}, expected {(S or B, H)}")
     _on_cuda(first, names[0])
     return [_rows(t) for t in tensors], h0, seq_starts, (B, T, H, S)
@@ -751,47 +787,49 @@ def _scan_operands(names, tensors, h0, seq_starts):
 
 def _check_decay(decay, device, H: int, scale: float) -> torch.Tensor:
     decay = _as_f32(decay, device, "decay")
-    if tuple(decay.shape) != (H,):
+    if decay.shape != (H,):
         raise ValueError(f"decay has shape {tuple(decay.shape)}, expected {(H,)}")
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale must be positive and finite (got {scale})")
     return decay
 
 
+def _scan_forward(decay, h0, seq_starts, dims, scale, keep, inputs):
+    """(h, h_final, what a backward needs besides the operands; ``keep``: one follows)."""
+    lib = _require_kernels()
+    B, T, H, S = dims
+    first = inputs[0]
+    dev, dtype = first.device, first.dtype
+    h = torch.empty(first.shape, device=dev, dtype=dtype)
+    h_final = torch.empty(S or B, H, device=dev, dtype=torch.float32)
+    if first.numel() == 0:
+        h_final.zero_() if h0 is None else h_final.copy_(h0)
+        return h, h_final, None
+    code = _DTYPES[dtype]
+    with _OnDevice(dev):
+        saved_bytes, ws_bytes, _ = _scan_plan(dev.index, dims, code)
+        saved = torch.empty(saved_bytes, device=dev, dtype=torch.uint8) if keep and saved_bytes else None
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
+        ins = [ctypes.byref(_scan_input(t)) for t in inputs]
+        tail = (_ptr(h0), _ptr(seq_starts), h.data_ptr(), h_final.data_ptr(), _ptr(saved), _ptr(ws), ws_bytes,
+                _current_stream(dev))
+        cd = ctypes.byref(LtcScanDims(B, T, H, code, S))
+        if decay is None:
+            _check(lib.ltc_linear_scan_forward(cd, *ins, *tail), "ltc_linear_scan")
+        else:
+            _check(lib.ltc_gated_scan_forward(cd, *ins, decay.data_ptr(), scale, *tail), "ltc_gated_scan")
+    return h, h_final, saved
+
+
 class _ScanFunction(torch.autograd.Function):
     """Both scans: ``inputs`` are (a, b), or (x, rate, gate) with ``decay``."""
 
     @staticmethod
-    def forward(ctx, decay, h0, seq_starts, dims, scale, needs_grad, *inputs):
-        lib = _require_kernels()
-        B, T, H, S = dims
-        first = inputs[0]
-        dev = first.device
+    def forward(ctx, decay, h0, seq_starts, dims, scale, *inputs):
+        h, h_final, saved = _scan_forward(decay, h0, seq_starts, dims, scale, True, inputs)
         ctx.dims, ctx.scale = dims, scale
         ctx.set_materialize_grads(False)
-        h = torch.empty(first.shape, device=dev, dtype=first.dtype)
-        h_final = torch.empty(S or B, H, device=dev, dtype=torch.float32)
-        saved = None
-        if first.numel() == 0:
-            h_final.zero_() if h0 is None else h_final.copy_(h0)
-        else:
-            cd = LtcScanDims(B, T, H, _DTYPES[first.dtype], S)
-            ins = [ctypes.byref(_scan_input(t)) for t in inputs]
-            with torch.cuda.device(dev):
-                p = LtcScanPlan()
-                _check(lib.ltc_scan_plan(ctypes.byref(cd), ctypes.byref(p)), "ltc_scan_plan")
-                if needs_grad and p.saved_bytes:
-                    saved = torch.empty(p.saved_bytes, device=dev, dtype=torch.uint8)
-                ws = torch.empty(p.fwd_workspace_bytes, device=dev, dtype=torch.uint8)
-                tail = (_ptr(h0), _ptr(seq_starts), h.data_ptr(), h_final.data_ptr(), _ptr(saved), _ptr(ws),
-                        p.fwd_workspace_bytes, _current_stream(dev))
-                if decay is None:
-                    _check(lib.ltc_linear_scan_forward(ctypes.byref(cd), *ins, *tail), "ltc_linear_scan")
-                else:
-                    _check(lib.ltc_gated_scan_forward(ctypes.byref(cd), *ins, decay.data_ptr(), scale, *tail),
-                           "ltc_gated_scan")
-        if needs_grad:
-            ctx.save_for_backward(decay, h0, seq_starts, saved, *inputs)
+        ctx.save_for_backward(decay, h0, seq_starts, saved, *inputs)
         return h, h_final
 
     @staticmethod
@@ -810,30 +848,36 @@ class _ScanFunction(torch.autograd.Function):
                 dh0.zero_() if dh_final is None else dh0.copy_(dh_final)
             if ddecay is not None:
                 ddecay.zero_()
-            return (ddecay, dh0, None, None, None, None, *grads)
+            return (ddecay, dh0, None, None, None, *grads)
         if dh is not None:
             dh = _rows(dh.to(first.dtype))
+            dh = dh if dh.stride(-2) <= SCAN_MAX_H else dh.contiguous()
         if dh_final is not None:
             dh_final = dh_final.to(torch.float32).contiguous()
         cd = LtcScanDims(B, T, H, _DTYPES[first.dtype], S)
         ins = [ctypes.byref(_scan_input(t)) for t in inputs]
-        with torch.cuda.device(dev):
-            p = LtcScanPlan()
-            _check(lib.ltc_scan_plan(ctypes.byref(cd), ctypes.byref(p)), "ltc_scan_plan")
-            ws = torch.empty(p.bwd_workspace_bytes, device=dev, dtype=torch.uint8)
+        with _OnDevice(dev):
+            _, _, ws_bytes = _scan_plan(dev.index, ctx.dims, cd.dtype)
+            ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
             mid = (_ptr(h0), _ptr(seq_starts), _ptr(saved), None if dh is None else ctypes.byref(_scan_input(dh)),
                    _ptr(dh_final), *[g.data_ptr() for g in grads])
-            tail = (_ptr(dh0), ws.data_ptr(), p.bwd_workspace_bytes, _current_stream(dev))
+            tail = (_ptr(dh0), ws.data_ptr(), ws_bytes, _current_stream(dev))
             if decay is None:
                 _check(lib.ltc_linear_scan_backward(ctypes.byref(cd), *ins, *mid, *tail), "ltc_linear_scan backward")
             else:
                 _check(lib.ltc_gated_scan_backward(ctypes.byref(cd), *ins, decay.data_ptr(), ctx.scale, *mid,
                                                    ddecay.data_ptr(), *tail), "ltc_gated_scan backward")
-        return (ddecay, dh0, None, None, None, None, *grads)
+        return (ddecay, dh0, None, None, None, *grads)
 
 
 def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _scan(decay, h0, seq_starts, dims, scale, inputs):
+    if _wants_grad(*inputs, decay, h0):
+        return _ScanFunction.apply(decay, h0, seq_starts, dims, scale, *inputs)
+    return _scan_forward(decay, h0, seq_starts, dims, scale, False, inputs)[:2]
 
 
 def ltc_linear_scan(a, b, h0=None, seq_starts=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -846,7 +890,7 @@ def ltc_linear_scan(a, b, h0=None, seq_starts=None) -> Tuple[torch.Tensor, torch
     between.  Tokens that belong to no sequence give 0 and get no gradient; a sequence
     without tokens returns its ``h0``.  Differentiable once in ``a``, ``b`` and ``h0``."""
     tensors, h0, seq_starts, dims = _scan_operands(("a", "b"), (a, b), h0, seq_starts)
-    return _ScanFunction.apply(None, h0, seq_starts, dims, 0.0, _wants_grad(*tensors, h0), *tensors)
+    return _scan(None, h0, seq_starts, dims, 0.0, tensors)
 
 
 def ltc_gated_scan(x, rate, gate, decay, h0=None, seq_starts=None, scale: float = 8.0):
@@ -860,7 +904,7 @@ def ltc_gated_scan(x, rate, gate, decay, h0=None, seq_starts=None, scale: float 
     inside the scan.  Differentiable once in all of them and ``h0``."""
     tensors, h0, seq_starts, dims = _scan_operands(("x", "rate", "gate"), (x, rate, gate), h0, seq_starts)
     decay = _check_decay(decay, tensors[0].device, dims[2], scale)
-    return _ScanFunction.apply(decay, h0, seq_starts, dims, float(scale), _wants_grad(*tensors, decay, h0), *tensors)
+    return _scan(decay, h0, seq_starts, dims, float(scale), tensors)
 
 
 def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_state=None):
@@ -872,10 +916,8 @@ def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_sta
     if first.dim() != 2:
         raise ValueError(f"x must be (B, H), got shape {tuple(first.shape)}")
     dev, (B, H) = first.device, first.shape
-    for t, n in ((rate, "rate"), (gate, "gate")):
-        _typed(t, n, first.dtype, dev)
-        if t.shape != first.shape:
-            raise ValueError(f"{n} has shape {tuple(t.shape)}, expected {tuple(first.shape)}")
+    _alike(rate, "rate", first)
+    _alike(gate, "gate", first)
     _on_cuda(first, "x")
     decay = _check_decay(decay, dev, H, scale)
     s = _as_f32(state, dev, "state")
@@ -895,7 +937,7 @@ def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_sta
     if h.numel():
         cd = LtcScanDims(B, 1, H, _DTYPES[first.dtype], 0)
         ins = [ctypes.byref(_scan_input(_rows(t))) for t in (x, rate, gate)]
-        with torch.cuda.device(dev):
+        with _OnDevice(dev):
             _check(lib.ltc_gated_scan_step(ctypes.byref(cd), *ins, decay.data_ptr(), float(scale), s.data_ptr(),
                                            h.data_ptr(), out_state.data_ptr(), _current_stream(dev)),
                    "ltc_gated_scan_step")
@@ -920,6 +962,10 @@ def _logits_operand(logits, temperature: float):
     if not 0.0 < temperature < 1e30:
         raise ValueError(f"temperature must be positive (got {temperature})")
     _on_cuda(logits, "logits")
+    if logits.is_contiguous():
+        V = logits.shape[-1]
+        rows = logits.numel() // V
+        return logits, (rows, max(1, rows), 0, V, V, _DTYPES[logits.dtype], temperature)
     z = _rows(logits)
     lead = [(n, st) for n, st in zip(z.shape[:-1], z.stride()[:-1]) if n != 1]
     merged = []  # outer to inner; neighbours that one stride walks are one
@@ -942,7 +988,7 @@ def _id_operand(t, name: str, device, shape) -> torch.Tensor:
         raise TypeError(f"{name} must be an int32 or int64 tensor")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     return t.to(torch.int64).contiguous()
 
@@ -957,22 +1003,27 @@ def _row_grad(g: Optional[torch.Tensor], rows: int):
     return g.contiguous(), 1
 
 
+def _distill_forward(z, ids, teacher, desc, keep):
+    """(loss, teacher probabilities and row statistics for a backward)"""
+    lib = _require_kernels()
+    dev, rows, K = z.device, desc[0], ids.shape[-1]
+    loss = torch.empty(z.shape[:-1], device=dev, dtype=torch.float32)
+    probs = torch.empty(rows, K, device=dev, dtype=torch.float32) if keep else None
+    stats = torch.empty(rows, 4, device=dev, dtype=torch.float32) if keep else None
+    if rows:
+        with _OnDevice(dev):
+            _check(lib.ltc_distill_forward(ctypes.byref(LtcLogits(z.data_ptr(), *desc)), ids.data_ptr(),
+                                           teacher.data_ptr(), _DTYPES[teacher.dtype], K, loss.data_ptr(),
+                                           _ptr(probs), _ptr(stats), _current_stream(dev)), "ltc_distill_loss")
+    return loss, probs, stats
+
+
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, ids, teacher, desc, needs_grad):
-        lib = _require_kernels()
-        dev, rows, K = z.device, desc[0], ids.shape[-1]
+    def forward(ctx, z, ids, teacher, desc):
+        loss, probs, stats = _distill_forward(z, ids, teacher, desc, True)
         ctx.desc = desc
-        loss = torch.empty(z.shape[:-1], device=dev, dtype=torch.float32)
-        probs = torch.empty(rows, K, device=dev, dtype=torch.float32) if needs_grad else None
-        stats = torch.empty(rows, 4, device=dev, dtype=torch.float32) if needs_grad else None
-        if rows:
-            with torch.cuda.device(dev):
-                _check(lib.ltc_distill_forward(ctypes.byref(LtcLogits(z.data_ptr(), *desc)), ids.data_ptr(),
-                                               teacher.data_ptr(), _DTYPES[teacher.dtype], K, loss.data_ptr(),
-                                               _ptr(probs), _ptr(stats), _current_stream(dev)), "ltc_distill_loss")
-        if needs_grad:
-            ctx.save_for_backward(z, ids, probs, stats)
+        ctx.save_for_backward(z, ids, probs, stats)
         return loss
 
     @staticmethod
@@ -983,12 +1034,12 @@ class _DistillLoss(torch.autograd.Function):
         dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
         g, stride = _row_grad(g, ctx.desc[0])
         if ctx.desc[0]:
-            with torch.cuda.device(z.device):
+            with _OnDevice(z.device):
                 _check(lib.ltc_distill_backward(ctypes.byref(LtcLogits(z.data_ptr(), *ctx.desc)), ids.data_ptr(),
                                                 ids.shape[-1], probs.data_ptr(), stats.data_ptr(), g.data_ptr(),
                                                 stride, dz.data_ptr(), _current_stream(z.device)),
                        "ltc_distill_loss backward")
-        return dz, None, None, None, None
+        return dz, None, None, None
 
 
 def ltc_distill_loss(logits, teacher_ids, teacher_logits, temperature: float = 1.0) -> torch.Tensor:
@@ -1010,7 +1061,9 @@ def ltc_distill_loss(logits, teacher_ids, teacher_logits, temperature: float = 1
         raise ValueError(f"teacher_logits has shape {tuple(shape)}, expected {tuple(z.shape[:-1])} + (K,) "
                          f"with 1 <= K <= {DISTILL_MAX_K}")
     ids = _id_operand(teacher_ids, "teacher_ids", z.device, shape)
-    return _DistillLoss.apply(z, ids, teacher_logits.detach().contiguous(), desc, _wants_grad(z))
+    teacher = teacher_logits.detach().contiguous()
+    return _DistillLoss.apply(z, ids, teacher, desc) if _wants_grad(z) else _distill_forward(z, ids, teacher, desc,
+                                                                                             False)[0]
 
 
 class TokenLogprobs(NamedTuple):
@@ -1020,27 +1073,32 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: Optional[torch.Tensor]
 
 
+def _token_logprobs_forward(z, tokens, desc, top_k, keep):
+    """(log probabilities, entropies, top ids and log probabilities, row statistics for a backward)"""
+    lib = _require_kernels()
+    dev, rows, lead = z.device, desc[0], z.shape[:-1]
+    lp = torch.empty(lead, device=dev, dtype=torch.float32)
+    ent = torch.empty(lead, device=dev, dtype=torch.float32)
+    stats = torch.empty(rows, 4, device=dev, dtype=torch.float32) if keep else None
+    top_ids = torch.empty(*lead, top_k, device=dev, dtype=torch.int64) if top_k else None
+    top_lp = torch.empty(*lead, top_k, device=dev, dtype=torch.float32) if top_k else None
+    if rows:
+        with _OnDevice(dev):
+            _check(lib.ltc_token_logprobs_forward(ctypes.byref(LtcLogits(z.data_ptr(), *desc)), tokens.data_ptr(),
+                                                  top_k, lp.data_ptr(), ent.data_ptr(), _ptr(top_ids), _ptr(top_lp),
+                                                  _ptr(stats), _current_stream(dev)), "ltc_token_logprobs")
+    return lp, ent, top_ids, top_lp, stats
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, tokens, desc, top_k, needs_grad):
-        lib = _require_kernels()
-        dev, rows, lead = z.device, desc[0], z.shape[:-1]
+    def forward(ctx, z, tokens, desc, top_k):
+        lp, ent, top_ids, top_lp, stats = _token_logprobs_forward(z, tokens, desc, top_k, True)
         ctx.desc = desc
         ctx.set_materialize_grads(False)
-        lp = torch.empty(lead, device=dev, dtype=torch.float32)
-        ent = torch.empty(lead, device=dev, dtype=torch.float32)
-        stats = torch.empty(rows, 4, device=dev, dtype=torch.float32) if needs_grad else None
-        top_ids = torch.empty(*lead, top_k, device=dev, dtype=torch.int64)
-        top_lp = torch.empty(*lead, top_k, device=dev, dtype=torch.float32)
-        if rows:
-            with torch.cuda.device(dev):
-                _check(lib.ltc_token_logprobs_forward(ctypes.byref(LtcLogits(z.data_ptr(), *desc)), tokens.data_ptr(),
-                                                      top_k, lp.data_ptr(), ent.data_ptr(), top_ids.data_ptr(),
-                                                      top_lp.data_ptr(), _ptr(stats), _current_stream(dev)),
-                       "ltc_token_logprobs")
-        if needs_grad:
-            ctx.save_for_backward(z, tokens, stats)
-        ctx.mark_non_differentiable(top_ids, top_lp)
+        ctx.save_for_backward(z, tokens, stats)
+        if top_k:
+            ctx.mark_non_differentiable(top_ids, top_lp)
         return lp, ent, top_ids, top_lp
 
     @staticmethod
@@ -1053,12 +1111,12 @@ class _TokenLogprobs(torch.autograd.Function):
         g_lp, lp_stride = _row_grad(g_lp, rows)
         g_ent, ent_stride = _row_grad(g_ent, rows)
         if rows:
-            with torch.cuda.device(z.device):
+            with _OnDevice(z.device):
                 _check(lib.ltc_token_logprobs_backward(ctypes.byref(LtcLogits(z.data_ptr(), *ctx.desc)),
                                                        tokens.data_ptr(), stats.data_ptr(), _ptr(g_lp), lp_stride,
                                                        _ptr(g_ent), ent_stride, dz.data_ptr(),
                                                        _current_stream(z.device)), "ltc_token_logprobs backward")
-        return dz, None, None, None, None
+        return dz, None, None, None
 
 
 def ltc_token_logprobs(logits, tokens, top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
@@ -1077,5 +1135,6 @@ def ltc_token_logprobs(logits, tokens, top_k: int = 0, temperature: float = 1.0)
     top_k = int(top_k)
     if not 0 <= top_k <= min(TOKEN_LOGPROBS_MAX_TOP, z.shape[-1]):
         raise ValueError(f"top_k must be between 0 and min({TOKEN_LOGPROBS_MAX_TOP}, V) (got {top_k})")
-    lp, ent, ids, best = _TokenLogprobs.apply(z, tok, desc, top_k, _wants_grad(z))
-    return TokenLogprobs(lp, ent, ids if top_k else None, best if top_k else None)
+    if _wants_grad(z):
+        return TokenLogprobs(*_TokenLogprobs.apply(z, tok, desc, top_k))
+    return TokenLogprobs(*_token_logprobs_forward(z, tok, desc, top_k, False)[:4])

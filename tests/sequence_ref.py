@@ -134,11 +134,11 @@ def scan_reference(op, args, h0, dh=None, dlast=None, starts=None, scale=8.0, dt
             for n, (v, e) in res.items()}
 
 
-def vocab_reference(kind, z, tau, V_threads=256, **kw):
+def vocab_reference(kind, z, tau, V_threads=128, **kw):
     """Distillation (ids, teacher) or token scores (tokens); fp64 values and bounds.
 
     y = (z - m) / (tau ln 2) is off by 3 U |y| (difference, two roundings of the factor);
-    2^y by that times ln 2 and 2 ulp; the sum of n = V / 256 + 16 additions in a row by n U of
+    2^y by that times ln 2 and 2 ulp; the sum of n = V / 128 + 16 additions in a row by n U of
     itself.  So log2 s is off by S = (4 U + n U) / ln 2 + 3 U E|y| with E over q, and a rounding of
     itself, log q by ln 2 (3 U |y| + S + U log2 s) + 2 U |log q|."""
     z = z.detach().cpu().double()

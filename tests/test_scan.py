@@ -59,12 +59,12 @@ def test_padded(op, B, T, H, dtype):
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("op", ["linear", "gated"])
 @pytest.mark.parametrize("H", [8, 7])
-def test_segments(op, H, dtype):
-    """Few chains: time is cut into segments."""
+def test_clusters(op, H, dtype):
+    """Few chains: a cluster of blocks takes each."""
     dims = ltc_cuda.LtcScanDims(1, 1500, H, 0, 0)
     p = ltc_cuda.LtcScanPlan()
     import ctypes
-    assert ltc_cuda._lib.ltc_scan_plan(ctypes.byref(dims), ctypes.byref(p)) == 0 and p.segments > 1
+    assert ltc_cuda._lib.ltc_scan_plan(ctypes.byref(dims), ctypes.byref(p)) == 0 and p.cluster > 1
     args, h0, dh, dlast = make(op, (1, 1500), H, dtype, H, 1)
     check(op, args, h0, dh, dlast, dtype)
 

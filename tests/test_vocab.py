@@ -325,7 +325,8 @@ def test_empty():
 
 
 def test_offsets_past_32_bits():
-    """More than 2^31 logits: the last rows against the same rows alone."""
+    """More than 2^31 logits: the last rows against the same rows alone, which are summed in another
+    order (n = V / 128 + 16 additions: 530 U = 3e-5), so that a gradient may round the other way."""
     rows, V = 32800, 65536
     z = torch.empty(rows, V, device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator("cuda").manual_seed(1))
     tok = torch.arange(rows, device="cuda") % V
@@ -335,8 +336,9 @@ def test_offsets_past_32_bits():
     tail = z.detach()[-600:].clone().requires_grad_(True)
     s = ltc_cuda.ltc_token_logprobs(tail, tok[-600:])
     (gt,) = torch.autograd.grad(s.logprobs.sum(), tail)
-    assert torch.equal(r.logprobs[-600:], s.logprobs) and torch.equal(r.entropy[-600:], s.entropy)
-    assert torch.equal(g[-600:], gt)
+    assert torch.allclose(r.logprobs[-600:], s.logprobs, rtol=0, atol=6e-5)
+    assert torch.allclose(r.entropy[-600:], s.entropy, rtol=0, atol=6e-4)
+    assert torch.allclose(g[-600:].float(), gt.float(), rtol=2 * 2.0 ** -7, atol=0)
 
 
 def test_streams_and_graphs():
