@@ -346,7 +346,7 @@ int ltc_timing_collect(double* total_ms, int32_t* launches, int n);
 int64_t ltc_launch_count(void);
 
 /* Number of bounded in-kernel waits (the per-unfold exchange between the CTAs
- * of a cluster, H in 65..128) that expired on the current device since the
+ * of a cluster, H in 65..128; the scans' exchange between the CTAs of one) that expired on the current device since the
  * library was loaded; 0 in a healthy process.  Synchronises with the device.
  * Returns -1 on a CUDA error. */
 int ltc_wait_timeouts(void);

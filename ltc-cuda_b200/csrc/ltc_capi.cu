@@ -391,9 +391,11 @@ int ltc_check_errors(int* count, int* first_site) {
 }
 
 int ltc_wait_timeouts(void) {
-  int n = 0, m = 0;
-  if (ltc::read_wait_timeouts(&n) != 0 || ltc::read_stream_wait_timeouts(&m) != 0) return -1;
-  return n + m;
+  int n = 0, m = 0, k = 0;
+  if (ltc::read_wait_timeouts(&n) != 0 || ltc::read_stream_wait_timeouts(&m) != 0 ||
+      ltc::read_scan_wait_timeouts(&k) != 0)
+    return -1;
+  return n + m + k;
 }
 
 int64_t ltc_launch_count(void) {
@@ -902,7 +904,7 @@ int scan_begin(const LtcScanDims* d, const char* who, ScanCall* c) {
   if (err) return 1;
   c->plan = plan_scan(d->B, d->T, d->H, d->num_seqs > 0, c->di.sms);
   const size_t bh = (size_t)d->B * d->H;
-  c->part_floats = bh * c->plan.cl;
+  c->part_floats = bh * c->plan.cl_bwd;
   c->saved_floats = bh * c->plan.nbounds;
   return 0;
 }
@@ -934,7 +936,7 @@ int scan_args(const LtcScanDims* d, const ScanCall& c, const char* who, const Lt
   a->h0 = h0;
   a->starts = starts;
   a->B = d->B; a->T = d->T; a->H = d->H; a->S = d->num_seqs;
-  a->nbounds = c.plan.nbounds; a->cl = c.plan.cl;
+  a->nbounds = c.plan.nbounds; a->cl = bwd ? c.plan.cl_bwd : c.plan.cl_fwd; a->narrow = c.plan.narrow;
   return 0;
 }
 
@@ -999,7 +1001,8 @@ int vocab_args(const LtcLogits* z, const char* who, VocabArgs* a, DeviceInfo* di
   if (z->rows < 1 || z->inner_rows < 1 || z->V < 1 || z->V > (1 << 30))
     return fail("%s: need rows, inner_rows >= 1 and 1 <= V <= 2^30", who);
   if (z->dtype < 0 || z->dtype > LTC_DTYPE_F16) return fail("%s: unknown dtype %d", who, z->dtype);
-  if (!(z->temperature > 0.f) || !(z->temperature < 1e30f)) return fail("%s: temperature must be positive", who);
+  if (!(z->temperature > 1e-30f) || !(z->temperature < 1e30f))
+    return fail("%s: temperature must be between 1e-30 and 1e30", who);
   int err = 0;
   *di = device_info(&err);
   if (err) return 1;
@@ -1031,7 +1034,7 @@ int ltc_scan_plan(const LtcScanDims* dims, LtcScanPlan* out) {
   out->saved_bytes = c.saved_floats * sizeof(float);
   out->fwd_workspace_bytes = scan_workspace(c, false);
   out->bwd_workspace_bytes = scan_workspace(c, true);
-  out->cluster = c.plan.cl;
+  out->cluster = c.plan.cl_fwd;
   g_last_error.clear();
   return 0;
 }

@@ -157,6 +157,7 @@ cudaError_t launch_recurrent_bwd(const RecBwdArgs& a, const RecPlan& p, cudaStre
 // bounded cluster waits that expired on the current device (ltc_recurrent.cu)
 int read_wait_timeouts(int* count);
 int read_stream_wait_timeouts(int* count);  // ltc_recurrent_stream.cu
+int read_scan_wait_timeouts(int* count);    // ltc_scan.cu
 
 // ---- deterministic reductions and final gradient transforms --------------
 struct FinishArgs {
@@ -230,13 +231,15 @@ struct ScanArgs {
   int B, T, H, S;
   float scale;
   int nbounds, cl;          // ScanPlan
+  bool narrow;
   // set per launch
   int chb, rounds;          // items side by side; tiles a block walks
   long long items;
 };
 struct ScanPlan {
   int nbounds;  // saved states of a row
-  int cl;       // blocks of an item
+  int cl_fwd, cl_bwd;  // blocks of an item
+  bool narrow;  // items of 16 channels instead of 32
 };
 ScanPlan plan_scan(int B, int T, int H, bool packed, int num_sms);
 // policy 0: linear, 1: gated; dtype 0: fp32, 1: bf16, 2: fp16

@@ -16,8 +16,9 @@
 // threads marches over its tiles with the state in registers, so every input is read once;
 // the next tile's loads are in flight while this one is combined and written.  Where there
 // are too few items to fill the GPU, a cluster of up to 16 blocks takes one item, block r the
-// tiles r, r + cl, ...: the blocks' folds go to every block's shared memory, one cluster
-// barrier per round.  All orders are fixed: results do not depend on scheduling.
+// tiles r, r + cl, ...: every round the blocks' folds go to every block's shared memory as
+// messages that complete bytes on the receiver's mbarrier (bounded waits).  All orders are
+// fixed: results do not depend on scheduling.
 //
 // Backward.  The forward leaves the state before every 32nd token (fp32); the backward
 // rebuilds the states of a tile from it in registers instead of reading h, which is both
@@ -30,6 +31,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "ltc_cluster.cuh"
 #include "ltc_common.cuh"
 #include "ltc_internal.h"
 
@@ -40,7 +42,7 @@ namespace ltc {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kItem = 32;  // channels of an item: LX * VEC in every variant
+constexpr int kItem = 32;  // channels of an item, 16 in the narrow shapes
 
 // ---- element types -------------------------------------------------------------
 template <typename T, int VEC> struct Raw;  // VEC elements as loaded
@@ -237,6 +239,7 @@ struct Walk {
       count += __popc(__ballot_sync(0xffffffffu, le));
     }
     n = min(block + max(count - 1, 0), S - 1);
+    LTC_CHECK(n >= 0 && n < S, 901);
     s0 = __ldg(starts + n);
     s1 = __ldg(starts + n + 1);
   }
@@ -245,25 +248,25 @@ struct Walk {
     Marks m;
     if (!(s0 < tile_t0 && tile_t0 < s1)) find(tile_t0);
     if (s0 < tile_t0 && s1 > tile_t0 + TT && begin <= tile_t0 && end >= tile_t0 + TT) return m;
+    // tokens before the first sequence and behind the last, then the ends that lie among the thread's tokens
+    const int before = min(max(begin - t0, 0), R), behind = min(max(t0 + R - end, 0), R);
+    m.out = ((1u << before) - 1) | (((1u << behind) - 1) << (R - behind));
     int k = n, a = s0, b = s1;
-#pragma unroll 1
-    for (int j = 0; j < R; ++j) {
-      const int t = t0 + j;
-      while (t >= b && k + 1 < S) {
-        ++k;
-        a = b;
-        b = __ldg(starts + k + 1);
+    while (true) {
+      if (a < b) {
+        if (a >= t0 && a < t0 + R && a < end) {
+          if (!m.first) m.nf = k;
+          m.first |= 1u << (a - t0);
+        }
+        if (b > t0 && b <= t0 + R && b <= end) {
+          if (!m.last) m.nl = k;
+          m.last |= 1u << (b - 1 - t0);
+        }
       }
-      const bool in = t >= begin && t < end;
-      if (!in) m.out |= 1u << j;
-      if (in && t == a) {
-        if (!m.first) m.nf = k;
-        m.first |= 1u << j;
-      }
-      if (in && t + 1 == b) {
-        if (!m.last) m.nl = k;
-        m.last |= 1u << j;
-      }
+      if (b >= t0 + R || k + 1 >= S) break;
+      ++k;
+      a = b;
+      b = __ldg(starts + k + 1);
     }
     return m;
   }
@@ -277,10 +280,11 @@ template <bool PACKED> struct WalkOf { using type = NoWalk; };
 template <> struct WalkOf<true> { using type = Walk; };
 
 // ---- shapes ----------------------------------------------------------------------
-template <int VEC_, int R_, int TY_, int BB_>
+template <int VEC_, int R_, int TY_, int BB_, int ITEM_ = kItem>
 struct Shape {
   static constexpr int VEC = VEC_, R = R_, TY = TY_, BB = BB_;
-  static constexpr int LX = kItem / VEC;  // lanes side by side: one row of an item
+  static constexpr int ITEM = ITEM_;
+  static constexpr int LX = ITEM / VEC;   // lanes side by side: one row of an item
   static constexpr int GPW = 32 / LX;     // time groups inside a warp
   static constexpr int NW = TY / GPW;     // warps along time
   static constexpr int TT = TY * R;       // tokens of a tile
@@ -290,42 +294,84 @@ struct Shape {
   static_assert((R * VEC) % 2 == 0 && GPW <= 2, "pairs; one shuffle step");
 };
 
-// what the blocks of a cluster tell each other about one round, and the warps of a block
-template <int NW, int NF>
+// What the warps of a block, and the blocks of a cluster, tell each other about one round.
+template <int NW, int NF, bool MANY>
 struct alignas(16) Exchange {
   float w[2][NW][NF][kItem];   // per warp: A, then B (and C in the backward)
   int wf[2][NW];               // whether it holds a cut
-  float x[2][kScanMaxCluster][2][kItem];  // per block: A and B or C
-  int xf[2][kScanMaxCluster];
+  float2 x[2][MANY ? kScanMaxCluster : 1][kItem];  // per block: (A, B) or (A, C)
+  float xf[2][MANY ? kScanMaxCluster : 1];         // not 0: it holds a cut
+  unsigned long long bar[2];   // bytes of a round's messages
+  int aborted;
 };
+__device__ int g_scan_wait_timeouts = 0;
 
-// sends this block's fold (over its warps, in time order) to all blocks of the cluster, and waits for theirs
-template <bool PACKED, bool REVERSE, int NW, int NF>
-__device__ __forceinline__ void exchange(Exchange<NW, NF>& sh, int buf, int cl, int rank) {
-  __syncthreads();
+__device__ __forceinline__ int message_bytes(int cl) { return cl * (kItem * (int)sizeof(float2) + (int)sizeof(float)); }
+
+// before the first round: both slots expect the messages of all blocks
+template <int NW, int NF>
+__device__ __forceinline__ void exchange_begin(Exchange<NW, NF, true>& sh, int cl) {
   if (cl == 1) return;
-  cg::cluster_group c = cg::this_cluster();
-  if (threadIdx.x < kItem) {
-    const int ch = threadIdx.x;
-    float A = 1.f, B = 0.f;
-    int F = 0;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const int w = REVERSE ? NW - 1 - i : i;
-      const float wa = sh.w[buf][w][0][ch];
-      const bool cut = PACKED && sh.wf[buf][w] != 0;
-      B = flow<PACKED>(cut, wa, B, sh.w[buf][w][NF - 1][ch]);
-      A *= wa;
-      F |= cut;
+  if (threadIdx.x == 0) {
+    sh.aborted = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&sh.bar[i]), 1);
     }
-    for (int r = 0; r < cl; ++r) {
-      Exchange<NW, NF>* to = c.map_shared_rank(&sh, r);
-      to->x[buf][rank][0][ch] = A;
-      to->x[buf][rank][1][ch] = B;
-      if (PACKED && ch == 0) to->xf[buf][rank] = F;
-    }
+    mbar_init_fence();
+    for (int i = 0; i < 2; ++i) mbar_arm(smem_addr(&sh.bar[i]), message_bytes(cl));
   }
-  c.sync();
+  cg::this_cluster().sync();
+}
+
+// The warps' folds are in shared memory: makes them visible to the block and sends the block's
+// fold (in time order) to all blocks of the cluster, each warp to its share of them.  The
+// messages complete bytes on the receiver's barrier, so that no block waits for its own.
+template <bool PACKED, bool REVERSE, int NW, int NF, bool MANY>
+__device__ __forceinline__ void exchange_send(Exchange<NW, NF, MANY>& sh, int buf, int cl, int rank) {
+  __syncthreads();
+  if (!MANY || cl == 1) return;
+  const int ch = threadIdx.x & 31;  // a narrow item's upper half sends what nobody reads
+  float A = 1.f, B = 0.f;
+  int F = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const int w = REVERSE ? NW - 1 - i : i;
+    const float wa = sh.w[buf][w][0][ch];
+    const bool cut = PACKED && sh.wf[buf][w] != 0;
+    B = flow<PACKED>(cut, wa, B, sh.w[buf][w][NF - 1][ch]);
+    A *= wa;
+    F |= cut;
+  }
+  const unsigned to = smem_addr(&sh.x[buf][rank][ch]);
+  const unsigned tf = smem_addr(&sh.xf[buf][rank]), bar = smem_addr(&sh.bar[buf]);
+  for (int r = threadIdx.x / 32; r < cl; r += NW) {
+    const unsigned rbar = cluster_map(bar, r);
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(
+                     cluster_map(to, r)), "r"(__float_as_uint(A)), "r"(__float_as_uint(B)), "r"(rbar) : "memory");
+    if (ch == 0) st_async(cluster_map(tf, r), F ? 1.f : 0.f, rbar);
+  }
+}
+// Waits for the round's messages.  A block writes a slot again two rounds later, after it has
+// all messages of the round between, which every block sends behind a block barrier that
+// follows its reads of the slot.
+template <int NW, int NF, bool MANY>
+__device__ __forceinline__ void exchange_wait(Exchange<NW, NF, MANY>& sh, int buf, int cl, int phase) {
+  if (!MANY || cl == 1) return;
+  const unsigned bar = smem_addr(&sh.bar[buf]);
+  mbar_wait(bar, phase, &sh.aborted, &g_scan_wait_timeouts);
+  if (threadIdx.x == 0) mbar_arm(bar, message_bytes(cl));
+}
+
+// (A, B) of this thread's channels
+__device__ __forceinline__ void message(const float2* x, int lx, float& a, float& b) {
+  const float2 v = x[lx];
+  a = v.x;
+  b = v.y;
+}
+__device__ __forceinline__ void message(const float2* x, int lx, float2& a, float2& b) {
+  const float4 v = *reinterpret_cast<const float4*>(x + 2 * lx);
+  a = make_float2(v.x, v.z);
+  b = make_float2(v.y, v.w);
 }
 
 struct Item {
@@ -333,20 +379,20 @@ struct Item {
   int ch, rank;
   bool chok;
 };
-template <typename S>
+template <typename S, bool MANY>
 __device__ __forceinline__ Item item_of(const ScanArgs& g, bool& out) {
   Item it;
   long long i = (long long)blockIdx.x;
   it.rank = 0;
   if (S::BB > 1) {
     i = i * S::BB + threadIdx.x / (S::LX * S::TY);
-  } else if (g.cl > 1) {
+  } else if (MANY) {
     it.rank = (int)(i % g.cl);
     i /= g.cl;
   }
   out = S::BB > 1 && i >= g.items;
   it.b = i / g.chb;
-  it.ch = (int)(i % g.chb) * kItem + (int)(threadIdx.x % S::LX) * S::VEC;
+  it.ch = (int)(i % g.chb) * S::ITEM + (int)(threadIdx.x % S::LX) * S::VEC;
   it.chok = it.ch < g.H;
   return it;
 }
@@ -437,19 +483,25 @@ __device__ __forceinline__ void gates_bwd(const float (&x)[R], const float (&y)[
 }
 
 // ---- forward -----------------------------------------------------------------------
-template <int P, typename T, typename S, bool PACKED>
-__global__ void __launch_bounds__(S::THREADS, PACKED || (P && (sizeof(T) == 4 || S::VEC == 1)) ? 4 : 5) scan_fwd_kernel(ScanArgs g) {
-  static_assert(!PACKED || S::NW > 1, "the one-warp tiles do not look at cuts");
+// blocks that an SM's registers have to hold
+template <int P, typename T, typename S, bool MANY>
+constexpr int fwd_blocks() {
+  return MANY || (P && (sizeof(T) == 4 || S::VEC == 1)) ? 4 : 5;
+}
+
+template <int P, typename T, typename S, bool PACKED, bool MANY>
+__global__ void __launch_bounds__(S::THREADS, (fwd_blocks<P, T, S, MANY>())) scan_fwd_kernel(ScanArgs g) {
+  static_assert(!(PACKED || MANY) || S::NW > 1, "the one-warp tiles look at neither cuts nor other blocks");
   constexpr int NIN = P ? 3 : 2, VEC = S::VEC, R = S::R, NW = S::NW, LX = S::LX;
   using V = typename Chans<VEC>::type;
-  __shared__ Exchange<NW, 2> sh;
+  __shared__ Exchange<NW, 2, MANY> sh;
   const int lx = threadIdx.x % LX, ty = (threadIdx.x / LX) % S::TY;
   const int grp = ty % S::GPW, wt = ty / S::GPW;  // group in the warp, warp along time
   bool out_of_items;
-  const Item it = item_of<S>(g, out_of_items);
+  const Item it = item_of<S, MANY>(g, out_of_items);
   if (out_of_items) return;  // whole warps leave; no block barrier follows
   const long long b = it.b;
-  const int ch = it.ch, cl = S::BB > 1 ? 1 : g.cl;
+  const int ch = it.ch, cl = MANY ? g.cl : 1;
   const bool chok = it.chok;
   const int cr = chok ? ch : 0;  // lanes past the last channel read the first one and write nothing
 
@@ -457,7 +509,7 @@ __global__ void __launch_bounds__(S::THREADS, PACKED || (P && (sizeof(T) == 4 ||
   if (P) cu = vmap(load_f32<V>(g.decay + cr), [&](float d) { return rate_of(d, g.scale); });
   if (!PACKED && g.h0) carry = load_f32<V>(g.h0 + b * g.H + cr);
 
-  if (cl > 1) cg::this_cluster().sync();  // every block of the cluster runs before its memory is written
+  if constexpr (MANY) exchange_begin(sh, cl);
   int t0 = it.rank * S::TT + ty * R;
   const char* in[NIN];
   typename Raw<T, VEC>::type raw[NIN][R];
@@ -524,10 +576,6 @@ __global__ void __launch_bounds__(S::THREADS, PACKED || (P && (sizeof(T) == 4 ||
       }
     }
     Marks next;
-    if (PACKED && round + 1 < g.rounds) {
-      next = walk.template marks<R, S::TT>(t0 + cl * S::TT - ty * R, t0 + cl * S::TT);
-      if (next.first && g.h0) hz = load_f32<V>(g.h0 + (long long)next.nf * g.H + cr);
-    }
 
     // fold of this thread's tokens, over the warp, over the block
     V A, B, Ax = all_of<V>(1.f), Bx{};
@@ -553,13 +601,19 @@ __global__ void __launch_bounds__(S::THREADS, PACKED || (P && (sizeof(T) == 4 ||
         store(&sh.w[buf][wt][1][lx * VEC], B);
         if (PACKED && lx == 0) sh.wf[buf][wt] = F;
       }
-      exchange<PACKED, false>(sh, buf, cl, it.rank);
+      exchange_send<PACKED, false>(sh, buf, cl, it.rank);
+      if (PACKED && round + 1 < g.rounds) {  // while the messages are on their way
+        next = walk.template marks<R, S::TT>(t0 + cl * S::TT - ty * R, t0 + cl * S::TT);
+        if (next.first && g.h0) hz = load_f32<V>(g.h0 + (long long)next.nf * g.H + cr);
+      }
+      exchange_wait(sh, buf, cl, (round >> 1) & 1);
       h = carry;
-      if (cl > 1) {
+      if (MANY && cl > 1) {
         for (int r = 0; r < cl; ++r) {
           if (r == it.rank) h = carry;
-          carry = flow<PACKED>(PACKED && sh.xf[buf][r] != 0, load_f32<V>(&sh.x[buf][r][0][lx * VEC]), carry,
-                               load_f32<V>(&sh.x[buf][r][1][lx * VEC]));
+          V xa, xb;
+          message(sh.x[buf][r], lx, xa, xb);
+          carry = flow<PACKED>(PACKED && sh.xf[buf][r] != 0.f, xa, carry, xb);
         }
       }
       V run = h;
@@ -624,31 +678,32 @@ __global__ void __launch_bounds__(S::THREADS, PACKED || (P && (sizeof(T) == 4 ||
 
 // blocks that an SM's registers have to hold; more spill (bf16 gated: 5 against 4 blocks 184 and 205 us at
 // 8 x 2048 x 2560, the second a partial wave of blocks; fp32 spills at 5: 242 against 195 us at 1 x 32771 x 512)
-template <int P, typename T, typename S, bool PACKED>
+template <int P, typename T, typename S, bool MANY>
 constexpr int bwd_blocks() {
-  if (!P) return PACKED || S::R * S::VEC > 8 ? 4 : 5;
+  if (MANY) return 3;
+  if (!P) return S::R * S::VEC > 8 ? 4 : 5;
   if (S::R * S::VEC > 8 || sizeof(T) == 4) return 3;
-  return PACKED ? 4 : 5;
+  return 5;
 }
 
 // ---- backward ----------------------------------------------------------------------
-template <int P, typename T, typename S, bool PACKED>
-__global__ void __launch_bounds__(S::THREADS, (bwd_blocks<P, T, S, PACKED>())) scan_bwd_kernel(ScanArgs g) {
-  static_assert(!PACKED || S::NW > 1, "the one-warp tiles do not look at cuts");
-  static_assert(S::NW == 1 || S::TT == kScanBound, "a tile starts at a saved state");
+template <int P, typename T, typename S, bool PACKED, bool MANY>
+__global__ void __launch_bounds__(S::THREADS, (bwd_blocks<P, T, S, MANY>())) scan_bwd_kernel(ScanArgs g) {
+  static_assert(!(PACKED || MANY) || S::NW > 1, "the one-warp tiles look at neither cuts nor other blocks");
+  static_assert(S::NW == 1 || S::TT % kScanBound == 0, "a tile starts at a saved state");
   constexpr int NIN = P ? 3 : 2, VEC = S::VEC, R = S::R, NW = S::NW, LX = S::LX;
   using V = typename Chans<VEC>::type;
-  __shared__ Exchange<NW, 3> sh;
+  __shared__ Exchange<NW, 3, MANY> sh;
   // what only the last step of a tile needs waits in shared memory, every thread in its own places, so that
   // five blocks fit an SM's registers instead of three
   __shared__ V parked[P ? 4 : 1][P ? R : 1][S::THREADS];
   const int lx = threadIdx.x % LX, ty = (threadIdx.x / LX) % S::TY;
   const int grp = ty % S::GPW, wt = ty / S::GPW;
   bool out_of_items;
-  const Item it = item_of<S>(g, out_of_items);
+  const Item it = item_of<S, MANY>(g, out_of_items);
   if (out_of_items) return;
   const long long b = it.b;
-  const int ch = it.ch, cl = S::BB > 1 ? 1 : g.cl;
+  const int ch = it.ch, cl = MANY ? g.cl : 1;
   const bool chok = it.chok;
   const int cr = chok ? ch : 0;
 
@@ -658,7 +713,7 @@ __global__ void __launch_bounds__(S::THREADS, (bwd_blocks<P, T, S, PACKED>())) s
   const V cn = vmul(cu, all_of<V>(-0.6931471805599453f));
   if (!PACKED && g.dhT) carry = load_f32<V>(g.dhT + b * g.H + cr);
 
-  if (cl > 1) cg::this_cluster().sync();
+  if constexpr (MANY) exchange_begin(sh, cl);
   int t0 = ((g.rounds - 1) * cl + it.rank) * S::TT + ty * R;
   const char* in[NIN + 1];
   typename Raw<T, VEC>::type raw[NIN + 1][R];
@@ -756,11 +811,6 @@ __global__ void __launch_bounds__(S::THREADS, (bwd_blocks<P, T, S, PACKED>())) s
     }
     const V h0f = hz;
     Marks next;
-    if (PACKED && round > 0) {
-      next = walk.template marks<R, S::TT>(t0 - cl * S::TT - ty * R, t0 - cl * S::TT);
-      if (next.first && g.h0) hz = load_f32<V>(g.h0 + (long long)next.nf * g.H + cr);
-      if (next.last && g.dhT) dz = load_f32<V>(g.dhT + (long long)next.nl * g.H + cr);
-    }
 
     // forward fold (A, B) and reverse fold (A, C) of this thread's tokens
     V A, B, C{};
@@ -788,20 +838,27 @@ __global__ void __launch_bounds__(S::THREADS, (bwd_blocks<P, T, S, PACKED>())) s
     }
     V c;
     if (NW > 1) {
-      const int buf = round & 1;
+      const int buf = (g.rounds - 1 - round) & 1;
       if (grp == 0) {
         store(&sh.w[buf][wt][0][lx * VEC], At);
         store(&sh.w[buf][wt][1][lx * VEC], Bt);
         store(&sh.w[buf][wt][2][lx * VEC], Ct);
         if (PACKED && lx == 0) sh.wf[buf][wt] = F | Fo;
       }
-      exchange<PACKED, true>(sh, buf, cl, it.rank);
+      exchange_send<PACKED, true>(sh, buf, cl, it.rank);
+      if (PACKED && round > 0) {
+        next = walk.template marks<R, S::TT>(t0 - cl * S::TT - ty * R, t0 - cl * S::TT);
+        if (next.first && g.h0) hz = load_f32<V>(g.h0 + (long long)next.nf * g.H + cr);
+        if (next.last && g.dhT) dz = load_f32<V>(g.dhT + (long long)next.nl * g.H + cr);
+      }
+      exchange_wait(sh, buf, cl, ((g.rounds - 1 - round) >> 1) & 1);
       c = carry;
-      if (cl > 1) {
+      if (MANY && cl > 1) {
         for (int r = cl - 1; r >= 0; --r) {
           if (r == it.rank) c = carry;
-          carry = flow<PACKED>(PACKED && sh.xf[buf][r] != 0, load_f32<V>(&sh.x[buf][r][0][lx * VEC]), carry,
-                               load_f32<V>(&sh.x[buf][r][1][lx * VEC]));
+          V xa, xb;
+          message(sh.x[buf][r], lx, xa, xb);
+          carry = flow<PACKED>(PACKED && sh.xf[buf][r] != 0.f, xa, carry, xb);
         }
       }
       V run = c;
@@ -966,7 +1023,7 @@ bool pairs_ok(const ScanArgs& a, int nin, int esize, bool bwd) {
 
 template <typename S, typename K>
 cudaError_t launch_one(K kernel, ScanArgs a, cudaStream_t st) {
-  a.chb = (a.H + kItem - 1) / kItem;
+  a.chb = (a.H + S::ITEM - 1) / S::ITEM;
   a.items = (long long)a.B * a.chb;
   if (S::BB > 1) a.cl = 1;
   const int tiles = (a.T + S::TT - 1) / S::TT;
@@ -995,40 +1052,45 @@ using FwdPair = Shape<2, 8, 8, 1>;
 using FwdOne = Shape<1, 16, 4, 1>;
 using BwdPair = Shape<2, 4, 8, 1>;
 using BwdOne = Shape<1, 8, 4, 1>;
+// 16 channels of twice the tokens: twice as many items where there are very few
+using FwdNarrow = Shape<1, 16, 8, 1, 16>;
+using BwdNarrow = Shape<1, 8, 8, 1, 16>;
+// rows of up to 16 and up to 8 tokens: a warp each
 using ShortPair = Shape<2, 8, 2, 4>;
 using ShortOne = Shape<1, 16, 1, 4>;
 using TinyPair = Shape<2, 4, 2, 4>;
 using TinyOne = Shape<1, 8, 1, 4>;
 
+template <int P, typename T, typename PAIR, typename ONE, bool PACKED, bool MANY>
+cudaError_t launch_dir(const ScanArgs& a, bool bwd, bool pair, cudaStream_t st) {
+  if (bwd)
+    return pair ? launch_one<PAIR>(scan_bwd_kernel<P, T, PAIR, PACKED, MANY>, a, st)
+                : launch_one<ONE>(scan_bwd_kernel<P, T, ONE, PACKED, MANY>, a, st);
+  return pair ? launch_one<PAIR>(scan_fwd_kernel<P, T, PAIR, PACKED, MANY>, a, st)
+              : launch_one<ONE>(scan_fwd_kernel<P, T, ONE, PACKED, MANY>, a, st);
+}
+template <int P, typename T, typename F, typename B, bool PACKED, bool MANY>
+cudaError_t launch_long(const ScanArgs& a, bool bwd, cudaStream_t st) {
+  if (bwd) return launch_one<B>(scan_bwd_kernel<P, T, B, PACKED, MANY>, a, st);
+  return launch_one<F>(scan_fwd_kernel<P, T, F, PACKED, MANY>, a, st);
+}
+
 template <int P, typename T>
 cudaError_t launch_typed(const ScanArgs& a, bool bwd, cudaStream_t st) {
   const bool pair = pairs_ok(a, P ? 3 : 2, (int)sizeof(T), bwd);
-  if (a.starts) {
-    if (bwd)
-      return pair ? launch_one<BwdPair>(scan_bwd_kernel<P, T, BwdPair, true>, a, st)
-                  : launch_one<BwdOne>(scan_bwd_kernel<P, T, BwdOne, true>, a, st);
-    return pair ? launch_one<FwdPair>(scan_fwd_kernel<P, T, FwdPair, true>, a, st)
-                : launch_one<FwdOne>(scan_fwd_kernel<P, T, FwdOne, true>, a, st);
-  }
-  if (a.T <= TinyPair::TT) {
-    if (bwd)
-      return pair ? launch_one<TinyPair>(scan_bwd_kernel<P, T, TinyPair, false>, a, st)
-                  : launch_one<TinyOne>(scan_bwd_kernel<P, T, TinyOne, false>, a, st);
-    return pair ? launch_one<TinyPair>(scan_fwd_kernel<P, T, TinyPair, false>, a, st)
-                : launch_one<TinyOne>(scan_fwd_kernel<P, T, TinyOne, false>, a, st);
-  }
-  if (a.T <= kScanShort) {
-    if (bwd)
-      return pair ? launch_one<ShortPair>(scan_bwd_kernel<P, T, ShortPair, false>, a, st)
-                  : launch_one<ShortOne>(scan_bwd_kernel<P, T, ShortOne, false>, a, st);
-    return pair ? launch_one<ShortPair>(scan_fwd_kernel<P, T, ShortPair, false>, a, st)
-                : launch_one<ShortOne>(scan_fwd_kernel<P, T, ShortOne, false>, a, st);
-  }
-  if (bwd)
-    return pair ? launch_one<BwdPair>(scan_bwd_kernel<P, T, BwdPair, false>, a, st)
-                : launch_one<BwdOne>(scan_bwd_kernel<P, T, BwdOne, false>, a, st);
-  return pair ? launch_one<FwdPair>(scan_fwd_kernel<P, T, FwdPair, false>, a, st)
-              : launch_one<FwdOne>(scan_fwd_kernel<P, T, FwdOne, false>, a, st);
+  if (a.narrow && (a.starts || a.T > kScanShort))
+    return a.starts ? launch_long<P, T, FwdNarrow, BwdNarrow, true, true>(a, bwd, st)
+                    : launch_long<P, T, FwdNarrow, BwdNarrow, false, true>(a, bwd, st);
+  if (a.starts)
+    return pair ? launch_long<P, T, FwdPair, BwdPair, true, true>(a, bwd, st)
+                : launch_long<P, T, FwdOne, BwdOne, true, true>(a, bwd, st);
+  if (a.T <= TinyPair::TT) return launch_dir<P, T, TinyPair, TinyOne, false, false>(a, bwd, pair, st);
+  if (a.T <= kScanShort) return launch_dir<P, T, ShortPair, ShortOne, false, false>(a, bwd, pair, st);
+  if (a.cl > 1)
+    return pair ? launch_long<P, T, FwdPair, BwdPair, false, true>(a, bwd, st)
+                : launch_long<P, T, FwdOne, BwdOne, false, true>(a, bwd, st);
+  return pair ? launch_long<P, T, FwdPair, BwdPair, false, false>(a, bwd, st)
+              : launch_long<P, T, FwdOne, BwdOne, false, false>(a, bwd, st);
 }
 
 template <int P>
@@ -1053,15 +1115,31 @@ cudaError_t launch_step(const ScanArgs& a, cudaStream_t st) {
 
 }  // namespace
 
+// Blocks of an item.  A block marches at the latency of its tiles, so few items are shared by
+// clusters until the SMs have a few blocks each (4 fit in the forward, 3 in the backward), the
+// smaller clusters first: their rounds are shorter.  Measured on a B200 with (items x blocks):
+// forward, 16387 packed tokens x 2048 bf16: 64 x 4 211 us, x 8 140, x 16 214 (a second wave);
+// 3 x 5000 x 1001 fp16: 96 x 4 35 us, x 8 37; both directions of 1 x 32771 x 512 fp32:
+// 16 x 16 240 us, 16 x 8 330, in narrow items 32 x 8 208, 32 x 16 240.
 ScanPlan plan_scan(int B, int T, int H, bool packed, int num_sms) {
   ScanPlan p;
   p.nbounds = (T - 1) / kScanBound;
-  const long long items = (long long)B * ((H + kItem - 1) / kItem);
-  p.cl = 1;
-  if (packed || T > kScanShort) {
-    const int tiles = (T + kScanBound - 1) / kScanBound;
-    while (p.cl < kScanMaxCluster && items * p.cl * 2 <= 5LL * num_sms && p.cl * 4 <= tiles) p.cl *= 2;
+  p.cl_fwd = p.cl_bwd = 1;
+  p.narrow = false;
+  if (!packed && T <= kScanShort) return p;
+  long long items = (long long)B * ((H + kItem - 1) / kItem);
+  if (8 * items < 2LL * num_sms) {
+    p.narrow = true;
+    items = (long long)B * ((H + kItem / 2 - 1) / (kItem / 2));
   }
+  auto blocks = [&](int tile, int fit) {
+    int cl = 1;
+    while (cl < 8 && items * cl * 2 <= (long long)fit * num_sms && cl * 2 * tile <= T) cl *= 2;
+    if (cl == 8 && items * 8 <= num_sms && 16 * tile <= T) cl = 16;
+    return cl;
+  };
+  p.cl_fwd = blocks(p.narrow ? FwdNarrow::TT : FwdPair::TT, 4);
+  p.cl_bwd = blocks(p.narrow ? BwdNarrow::TT : BwdPair::TT, 3);
   return p;
 }
 
@@ -1079,6 +1157,10 @@ cudaError_t launch_gated_step(const ScanArgs& a, int dtype, cudaStream_t st) {
     case 1: return launch_step<__nv_bfloat16>(a, st);
     default: return launch_step<__half>(a, st);
   }
+}
+
+int read_scan_wait_timeouts(int* count) {
+  return (int)cudaMemcpyFromSymbol(count, g_scan_wait_timeouts, sizeof(int));
 }
 
 }  // namespace ltc

@@ -441,7 +441,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
     float thr = top.warp_v[0];
 #pragma unroll
     for (int q = 1; q < NW; ++q) thr = fminf(thr, top.warp_v[q]);
-    if (thr == neg_inf() && t.m != neg_inf()) {  // short or masked rows leave a warp without values: the k-th largest thread maximum
+    if (thr == neg_inf() && t.m != neg_inf()) {
+      // short or masked rows leave a warp without values: the k-th largest thread maximum instead
       int above = 0;
       for (int d = 0; d < NT; ++d) above += better(top.thread_v[d], d, best, tid) ? 1 : 0;
       if (above == g.k - 1) top.thr = best;
@@ -451,6 +452,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
     auto reaches = [&](float v) { return v >= thr && v > neg_inf(); };
     auto keep = [&](float v, int i) {
       const int at = atomicAdd(&top.count, 1);  // the order in the list does not matter
+      LTC_CHECK(i >= 0 && i < g.V, 911);
       if (at < kCap) {
         top.cv[at] = v;
         top.ci[at] = i;
@@ -553,7 +555,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
     if (rank != 0) return;
     if constexpr (TOPK) select_best<NT>(top.cv, top.ci, cs * g.k, g.k, top.ov, top.oi);
   }
-  if (!DISTILL && warp * 32 >= max(entries, TOPK ? g.k : 0)) return;
+  if (!DISTILL && warp * 32 >= max(entries, TOPK ? g.k : 0)) return;  // no barrier follows
   const bool empty = t.m == neg_inf();
   const float l2 = empty ? 0.f : log2f(t.s);
 

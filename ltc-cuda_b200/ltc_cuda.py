@@ -867,6 +867,8 @@ class _ScanFunction(torch.autograd.Function):
             else:
                 _check(lib.ltc_gated_scan_backward(ctypes.byref(cd), *ins, decay.data_ptr(), ctx.scale, *mid,
                                                    ddecay.data_ptr(), *tail), "ltc_gated_scan backward")
+        if _CHECK_WAITS[0]:
+            _check_waits_after("scan backward")
         return (ddecay, dh0, None, None, None, *grads)
 
 
@@ -959,8 +961,8 @@ def _logits_operand(logits, temperature: float):
         raise ValueError(f"logits must be (..., V) with V >= 1, got shape {tuple(logits.shape)}")
     if logits.shape[-1] > 1 << 30:
         raise ValueError("the vocabulary has more than 2^30 entries")
-    if not 0.0 < temperature < 1e30:
-        raise ValueError(f"temperature must be positive (got {temperature})")
+    if not 1e-30 < temperature < 1e30:
+        raise ValueError(f"temperature must be between 1e-30 and 1e30 (got {temperature})")
     _on_cuda(logits, "logits")
     if logits.is_contiguous():
         V = logits.shape[-1]

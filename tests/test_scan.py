@@ -1,4 +1,6 @@
 """GPU: ltc_linear_scan, ltc_gated_scan and ltc_gated_scan_step against the fp64 recurrence."""
+import ctypes
+
 import pytest
 import torch
 
@@ -58,14 +60,13 @@ def test_padded(op, B, T, H, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("op", ["linear", "gated"])
-@pytest.mark.parametrize("H", [8, 7])
-def test_clusters(op, H, dtype):
-    """Few chains: a cluster of blocks takes each."""
-    dims = ltc_cuda.LtcScanDims(1, 1500, H, 0, 0)
+@pytest.mark.parametrize("B,T,H", [(1, 1500, 8), (1, 1500, 7), (1, 2300, 40), (3, 700, 600), (2, 400, 1301)])
+def test_clusters(op, B, T, H, dtype):
+    """Few chains: a cluster of blocks takes each, in narrow items where there are fewest."""
+    dims = ltc_cuda.LtcScanDims(B, T, H, 0, 0)
     p = ltc_cuda.LtcScanPlan()
-    import ctypes
     assert ltc_cuda._lib.ltc_scan_plan(ctypes.byref(dims), ctypes.byref(p)) == 0 and p.cluster > 1
-    args, h0, dh, dlast = make(op, (1, 1500), H, dtype, H, 1)
+    args, h0, dh, dlast = make(op, (B, T), H, dtype, H, B)
     check(op, args, h0, dh, dlast, dtype)
 
 
@@ -328,6 +329,50 @@ def test_streams_and_graphs():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(u, v) for u, v in zip(out, want))
+
+
+def test_captured_cluster_of_sixteen():
+    """The largest cluster (a launch attribute beyond the portable size), captured and replayed
+    twice on changed inputs, padded and packed."""
+    args, h0, dh, dlast = make("gated", (1, 4200), 16, torch.bfloat16, 31, 1)
+    new = make("gated", (1, 4200), 16, torch.bfloat16, 32, 1)
+    starts = torch.tensor([0, 100, 100, 4100], dtype=torch.int32, device="cuda")
+
+    def step(a, g, gl):
+        leaves = [t.detach().requires_grad_(True) for t in a.values()]
+        h, last = call("gated", dict(zip(a, leaves)), None)
+        flat = {n: t if n == "decay" else t[0] for n, t in zip(a, leaves)}
+        hp, lp = call("gated", flat, None, starts)
+        return [h.detach(), hp.detach(), lp.detach(), *torch.autograd.grad([h, last, hp], leaves, [g, gl, g[0]])]
+
+    step(args, dh, dlast)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(args, dh, dlast)
+    for t, n in zip([*args.values(), dh, dlast], [*new[0].values(), new[2], new[3]]):
+        t.copy_(n)
+    want = step(new[0], new[2], new[3])
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(out, want))
+
+
+def test_two_streams_at_once():
+    """Two scans in flight on two streams share nothing."""
+    jobs = [make(op, (2, 3000), 20, torch.float32, i, 2) for i, op in enumerate(("linear", "gated"))]
+    want = [call(op, j[0], j[1]) for op, j in zip(("linear", "gated"), jobs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = []
+    for _ in range(3):
+        for op, j, st in zip(("linear", "gated"), jobs, streams):
+            with torch.cuda.stream(st):
+                got.append(call(op, j[0], j[1]))
+    torch.cuda.synchronize()
+    for i, (h, last) in enumerate(got):
+        assert torch.equal(h, want[i % 2][0]) and torch.equal(last, want[i % 2][1])
 
 
 def test_solver_without_recurrent_synapses_is_a_linear_scan():

@@ -37,6 +37,7 @@ def t(*shape, dtype=torch.float32):
     (TypeError, lambda: ltc_cuda.ltc_distill_loss(t(2, 5, dtype=torch.int64), t(2, 1, dtype=torch.int64), t(2, 1))),
     (ValueError, lambda: ltc_cuda.ltc_distill_loss(t(2, 0), t(2, 1, dtype=torch.int64), t(2, 1))),
     (ValueError, lambda: ltc_cuda.ltc_distill_loss(t(2, 5), t(2, 1, dtype=torch.int64), t(2, 1), temperature=0.0)),
+    (ValueError, lambda: ltc_cuda.ltc_distill_loss(t(2, 5), t(2, 1, dtype=torch.int64), t(2, 1), temperature=1e-40)),
     (ValueError, lambda: ltc_cuda.ltc_token_logprobs(t(2, 5), t(2, dtype=torch.int64), temperature=float("nan"))),
     (ValueError, lambda: ltc_cuda.ltc_token_logprobs(t(2, 5), t(2, dtype=torch.int64))),
 ])
