@@ -136,18 +136,22 @@ __device__ __forceinline__ float rsqrt_ftz(float x) {
 __device__ __forceinline__ float2 ex2_2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
 __device__ __forceinline__ float2 rcp_2(float2 x) { return make_float2(rcp_approx(x.x), rcp_approx(x.y)); }
 
-// 1 - a^2 = 1 - exp(-y), y = 2 ln(2) u.  Near 0, where the difference cancels, the Taylor
-// series y - y^2/2 + ... in u, whose first left-out term is below 2^-24 of the sum for
-// y < 1/4; past it 1 - a^2 is at least 0.22.
-__device__ __forceinline__ float2 one_minus_sq(float2 a, float2 u) {
-  constexpr double c = 1.3862943611198906;  // 2 ln 2
-  float2 p = fma2(u, two((float)(-c * c * c * c * c * c / 720)), two((float)(c * c * c * c * c / 120)));
-  p = fma2(u, p, two((float)(-c * c * c * c / 24)));
-  p = fma2(u, p, two((float)(c * c * c / 6)));
-  p = fma2(u, p, two((float)(-c * c / 2)));
-  p = mul2(fma2(u, p, two((float)c)), u);
-  constexpr float limit = (float)(0.25 / c);
-  return make_float2(u.x < limit ? p.x : fmaf(-a.x, a.x, 1.f), u.y < limit ? p.y : fmaf(-a.y, a.y, 1.f));
+// a = 2^-u and om = 1 - a^2 = c (2 - c), c = 1 - a.  Near 1, where a step of a is a large part of
+// c and exp2's 2 ulp would shift the decay of a slow channel, c is the Taylor series y - y^2/2 +
+// ... of 1 - exp(-y), y = ln(2) u, whose first left-out term is below 2^-24 of the sum for
+// y < 1/4, and a its rounded complement; past it c is at least 0.22.
+__device__ __forceinline__ void decay_of(float2 u, float2& a, float2& om) {
+  constexpr double l = 0.6931471805599453;  // ln 2
+  float2 p = fma2(u, two((float)(-l * l * l * l * l * l / 720)), two((float)(l * l * l * l * l / 120)));
+  p = fma2(u, p, two((float)(-l * l * l * l / 24)));
+  p = fma2(u, p, two((float)(l * l * l / 6)));
+  p = fma2(u, p, two((float)(-l * l / 2)));
+  p = mul2(fma2(u, p, two((float)l)), u);
+  const float2 e = make_float2(ex2(-u.x), ex2(-u.y));
+  constexpr float limit = (float)(0.25 / l);
+  const float2 c = make_float2(u.x < limit ? p.x : 1.f - e.x, u.y < limit ? p.y : 1.f - e.y);
+  a = make_float2(u.x < limit ? 1.f - p.x : e.x, u.y < limit ? 1.f - p.y : e.y);
+  om = mul2(c, fma2(c, two(-1.f), two(2.f)));
 }
 
 __device__ __forceinline__ float softplus_of(float x) { return x > 20.f ? x : log1pf(expf(x)); }
@@ -160,8 +164,8 @@ __device__ __forceinline__ float rate_of(float decay, float scale) { return scal
 __device__ __forceinline__ void gate_fwd(float2 rate, float2 gate, float2 cu, float2& a, float2& w) {
   const float2 s = rcp_2(add2(ex2_2(mul2(rate, two(-kLog2e))), two(1.f)));
   const float2 u = mul2(cu, s);
-  a = make_float2(ex2(-u.x), ex2(-u.y));
-  const float2 om = one_minus_sq(a, u);
+  float2 om;
+  decay_of(u, a, om);
   const float2 pg = add2(ex2_2(mul2(gate, two(-kLog2e))), two(1.f));
   const float2 q = mul2(mul2(make_float2(fmaxf(om.x, kTinyOm), fmaxf(om.y, kTinyOm)), pg), pg);
   w = mul2(om, make_float2(rsqrt_ftz(q.x), rsqrt_ftz(q.y)));
@@ -172,8 +176,8 @@ __device__ __forceinline__ void gate_bwd(float2 x, float2 rate, float2 gate, flo
                                          float2& s, float2& b, float2& k, float2& m) {
   s = rcp_2(add2(ex2_2(mul2(rate, two(-kLog2e))), two(1.f)));
   const float2 u = mul2(cu, s);
-  a = make_float2(ex2(-u.x), ex2(-u.y));
-  const float2 om = one_minus_sq(a, u);
+  float2 om;
+  decay_of(u, a, om);
   const float2 sg = rcp_2(add2(ex2_2(mul2(gate, two(-kLog2e))), two(1.f)));
   const float2 rs = make_float2(rsqrt_ftz(fmaxf(om.x, kTinyOm)), rsqrt_ftz(fmaxf(om.y, kTinyOm)));
   w = mul2(mul2(om, rs), sg);
