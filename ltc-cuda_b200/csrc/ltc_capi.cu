@@ -894,8 +894,8 @@ struct ScanCall {
 
 int scan_begin(const LtcScanDims* d, const char* who, ScanCall* c) {
   if (!d) return fail("%s: dims is NULL", who);
-  if (d->B < 1 || d->T < 1 || d->H < 1 || d->T > 0x7fffff00)
-    return fail("%s: need B, T, H >= 1 (got %d, %d, %d)", who, d->B, d->T, d->H);
+  if (d->B < 1 || d->T < 1 || d->H < 1 || d->T > kScanMaxT)
+    return fail("%s: need B, T, H >= 1 and T <= %d (got %d, %d, %d)", who, kScanMaxT, d->B, d->T, d->H);
   if (d->dtype < 0 || d->dtype > LTC_DTYPE_F16) return fail("%s: unknown dtype %d", who, d->dtype);
   if (d->H > kScanMaxH) return fail("%s: at most %d channels", who, kScanMaxH);
   if (d->num_seqs < 0 || (d->num_seqs > 0 && d->B != 1)) return fail("%s: packed sequences need B = 1", who);

@@ -681,6 +681,7 @@ def ltc_preamble(x, ln_w, ln_b, in_w, in_b, eps: float):
 # Linear recurrences, parallel over time
 # ---------------------------------------------------------------------------
 SCAN_MAX_H = 1 << 28
+SCAN_MAX_T = 0x7fff0000
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -712,6 +713,11 @@ def _scan_input(t: torch.Tensor) -> LtcScanInput:
     if t.dim() == 3:
         return LtcScanInput(t.data_ptr(), t.stride(0), t.stride(1))
     return LtcScanInput(t.data_ptr(), t.stride(0), t.stride(0))
+
+
+def _fresh(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape, type and place (``empty_like`` is the cheaper call)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
 
 
 def _current_stream(dev) -> int:
@@ -775,8 +781,8 @@ def _scan_operands(names, tensors, h0, seq_starts):
         T, H = first.shape
         B, S = 1, seq_starts.numel() - 1
         seq_starts = seq_starts.to(torch.int32).contiguous()
-    if T > 0x7fffff00 or H > SCAN_MAX_H or any(t.stride(-2) > SCAN_MAX_H for t in tensors):
-        raise ValueError("more than 2^31 - 256 time steps, 2^28 channels, or a time stride past 2^28 elements")
+    if T > SCAN_MAX_T or H > SCAN_MAX_H or any(t.stride(-2) > SCAN_MAX_H for t in tensors):
+        raise ValueError("more than 2^31 - 2^16 time steps, 2^28 channels, or a time stride past 2^28 elements")
     if h0 is not None:
         h0 = _as_f32(h0, first.device, "h0")
         if h0.shape != (S or B, H):
@@ -800,8 +806,8 @@ def _scan_forward(decay, h0, seq_starts, dims, scale, keep, inputs):
     B, T, H, S = dims
     first = inputs[0]
     dev, dtype = first.device, first.dtype
-    h = torch.empty(first.shape, device=dev, dtype=dtype)
-    h_final = torch.empty(S or B, H, device=dev, dtype=torch.float32)
+    h = _fresh(first)
+    h_final = torch.empty(S or B, H, device=dev, dtype=torch.float32) if h0 is None else torch.empty_like(h0)
     if first.numel() == 0:
         h_final.zero_() if h0 is None else h_final.copy_(h0)
         return h, h_final, None
@@ -840,7 +846,7 @@ class _ScanFunction(torch.autograd.Function):
         B, T, H, S = ctx.dims
         first = inputs[0]
         dev = first.device
-        grads = [torch.empty(t.shape, device=dev, dtype=t.dtype) for t in inputs]
+        grads = [_fresh(t) for t in inputs]
         dh0 = None if h0 is None else torch.empty_like(h0)
         ddecay = None if decay is None else torch.empty_like(decay)
         if first.numel() == 0:
@@ -928,14 +934,14 @@ def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_sta
     if _wants_grad(x, rate, gate, decay, state):
         raise RuntimeError("ltc_gated_scan_step has no backward pass; use ltc_gated_scan or torch.no_grad()")
     if out_state is None:
-        out_state = torch.empty(B, H, device=dev, dtype=torch.float32)
+        out_state = torch.empty_like(s)
     elif (not isinstance(out_state, torch.Tensor) or out_state.dtype != torch.float32 or out_state.device != dev
           or out_state.shape != first.shape or not out_state.is_contiguous()):
         raise ValueError("out_state must be a contiguous fp32 tensor shaped and placed like x")
     elif 0 < abs(out_state.data_ptr() - s.data_ptr()) < 4 * s.numel():
         raise ValueError("out_state may be state itself but not overlap it otherwise")
     lib = _require_kernels()
-    h = torch.empty(B, H, device=dev, dtype=first.dtype)
+    h = _fresh(first)
     if h.numel():
         cd = LtcScanDims(B, 1, H, _DTYPES[first.dtype], 0)
         ins = [ctypes.byref(_scan_input(_rows(t))) for t in (x, rate, gate)]
@@ -1033,7 +1039,7 @@ class _DistillLoss(torch.autograd.Function):
     def backward(ctx, g):
         lib = _require_kernels()
         z, ids, probs, stats = ctx.saved_tensors
-        dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
+        dz = _fresh(z)
         g, stride = _row_grad(g, ctx.desc[0])
         if ctx.desc[0]:
             with _OnDevice(z.device):
@@ -1109,7 +1115,7 @@ class _TokenLogprobs(torch.autograd.Function):
         lib = _require_kernels()
         z, tokens, stats = ctx.saved_tensors
         rows = ctx.desc[0]
-        dz = torch.empty(z.shape, device=z.device, dtype=z.dtype)
+        dz = _fresh(z)
         g_lp, lp_stride = _row_grad(g_lp, rows)
         g_ent, ent_stride = _row_grad(g_ent, rows)
         if rows:

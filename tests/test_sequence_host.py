@@ -101,7 +101,7 @@ def test_c_entries_refuse_without_a_gpu():
         pytest.skip("library not built")
     p = ltc_cuda.LtcScanPlan()
     assert lib.ltc_scan_plan(None, ctypes.byref(p)) != 0
-    for bad in ((0, 1, 1, 0, 0), (1, 0, 1, 0, 0), (1, 1, 1, 3, 0), (2, 1, 1, 0, 1), (1, 1, 1, 0, -1)):
+    for bad in ((1, 0x7fff0001, 1, 0, 0), (1, 1, (1 << 28) + 1, 0, 0), (0, 1, 1, 0, 0), (1, 0, 1, 0, 0), (1, 1, 1, 3, 0), (2, 1, 1, 0, 1), (1, 1, 1, 0, -1)):
         assert lib.ltc_scan_plan(ctypes.byref(ltc_cuda.LtcScanDims(*bad)), ctypes.byref(p)) != 0
         assert lib.ltc_last_error()
     assert lib.ltc_gated_scan_step(None, None, None, None, None, 8.0, None, None, None, None) != 0
