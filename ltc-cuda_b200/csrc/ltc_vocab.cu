@@ -14,8 +14,8 @@
 // in shared memory over DSMEM, in rank order.  Bound by the one read of the logits.
 //
 // The k best ride in the same pass: every thread notes the maximum of each window of values it
-// reads.  Behind the pass a threshold that at least k thread maxima reach (the ceil(k/8)-th
-// largest of every warp, least over the 8 warps) leaves a few windows, whose values are read
+// reads.  Behind the pass a threshold that at least k thread maxima reach (the k-th largest of
+// the ceil(k / warps) + 1 largest of every warp) leaves a few windows, whose values are read
 // again; the few that reach the threshold are ranked by counting.  Where too many reach it (a
 // row of equal values, say) the row is searched k times instead: slow and right.  Ties go
 // to the lowest index.
@@ -245,6 +245,7 @@ struct TopShared {
   float ov[kVocabMaxTop];
   int oi[kVocabMaxTop];
   float thread_v[NT];
+  float best_v[kVocabMaxTop + 2 * (NT / 32)];
   float warp_v[NT / 32];
   int warp_i[NT / 32];
   int count;
@@ -384,17 +385,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
     if (DISTILL) warp_em[warp] = em;
   }
   if constexpr (TOPK) {
-    // the need-th largest maximum of each warp's threads
-    const int need = (g.k + NW - 1) / NW;
-    float x = best, w = neg_inf();
+    // the largest maxima of each warp's threads, at least k in all
+    const int need = (g.k + NW - 1) / NW + 1;
+    float x = best;
     for (int q = 0; q < need; ++q) {
-      w = x;
+      float w = x;
 #pragma unroll
       for (int d = 16; d >= 1; d >>= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, d));
       const unsigned who = __ballot_sync(0xffffffffu, x == w);
       if (lane == __ffs(who) - 1) x = neg_inf();
+      if (lane == 0) top.best_v[warp * need + q] = w;
     }
-    if (lane == 0) top.warp_v[warp] = w;
     top.thread_v[tid] = best;
     if (tid == 0) {
       top.count = 0;
@@ -405,6 +406,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
   Sums t{warp_m[0], 0.f, 0.f};
 #pragma unroll
   for (int w = 1; w < NW; ++w) t.m = max_nan(t.m, warp_m[w]);
+  if constexpr (TOPK) {  // the k-th largest of them: k values reach it
+    const int m = ((g.k + NW - 1) / NW + 1) * NW;
+    if (tid < m) {
+      const float v = top.best_v[tid];
+      int above = 0;
+      for (int d = 0; d < m; ++d) above += better(top.best_v[d], d, v, tid) ? 1 : 0;
+      if (above == g.k - 1) top.thr = v;
+    }
+  }
   float te[E], es = 0.f;  // this thread's entries up to their sum
   if constexpr (DISTILL) {
     em = warp_em[0];
@@ -438,11 +448,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
   }
 
   if constexpr (TOPK) {
-    float thr = top.warp_v[0];
-#pragma unroll
-    for (int q = 1; q < NW; ++q) thr = fminf(thr, top.warp_v[q]);
+    float thr = top.thr;
     if (thr == neg_inf() && t.m != neg_inf()) {
-      // short or masked rows leave a warp without values: the k-th largest thread maximum instead
+      // short or masked rows leave warps without values: the k-th largest of all thread maxima instead
       int above = 0;
       for (int d = 0; d < NT; ++d) above += better(top.thread_v[d], d, best, tid) ? 1 : 0;
       if (above == g.k - 1) top.thr = best;
