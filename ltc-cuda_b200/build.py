@@ -7,10 +7,12 @@ torch dependency (plain C-ABI over the CUDA runtime).
 from __future__ import annotations
 
 import argparse
+import concurrent.futures
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -44,19 +46,26 @@ def sources_newer_than_lib() -> bool:
 def build(force: bool = False, verbose_ptxas: bool = False, out: str = LIB, defines=()) -> str:
     if out == LIB and not force and not sources_newer_than_lib():
         return LIB
-    cmd = [nvcc_path(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "--expt-relaxed-constexpr", "-o", out + ".tmp"]
-    cmd += [f"-D{d}" for d in defines]
+    flags = [*ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
+    flags += [f"-D{d}" for d in defines]
     if verbose_ptxas:
-        cmd += ["-Xptxas", "-v"]
-    cmd += [os.path.join(CSRC, s) for s in SOURCES]
-    cmd += ["-lcudart"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError("nvcc failed building libltc_sm100.so")
-    if verbose_ptxas:
-        sys.stderr.write(r.stderr)
+        flags += ["-Xptxas", "-v"]
+    nvcc = nvcc_path()
+
+    def run(cmd):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            sys.stderr.write(r.stdout + r.stderr)
+            raise RuntimeError("nvcc failed building libltc_sm100.so")
+        if verbose_ptxas:
+            sys.stderr.write(r.stderr)
+
+    # one object per source, side by side: the kernel files take minutes each
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            list(pool.map(run, [[nvcc, *flags, "-c", "-o", o, os.path.join(CSRC, s)] for s, o in zip(SOURCES, objs)]))
+        run([nvcc, *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", out + ".tmp", *objs, "-lcudart"])
     os.replace(out + ".tmp", out)
     return out
 

@@ -273,13 +273,13 @@ __device__ __forceinline__ void load_window(uint4 (&r)[kUnroll], const Part<T>& 
 #pragma unroll
   for (int k = 0; k < kUnroll; ++k)
     r[k] = k * NT < left ? __ldg(pv + k * NT)
-                               : make_uint4(Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf);
+                         : make_uint4(Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf);
 }
 
 // ---- forward -----------------------------------------------------------------------
-// A block or cluster per row; reads of one block run while others compute (persistent blocks that
-// fetch the next window ahead hold 64 registers instead of 48 and were slower: 87 against 72 us at
-// 4096 x 32768 bf16).
+// A block or cluster per row; reads of one block run while others compute.  (Persistent blocks
+// whose next windows are on their way, in registers or a cp.async ring, were slower: 87 and 75
+// against 72 us at 4096 x 32768 bf16, before the reductions became cheaper: 64 now.)
 template <typename T, bool DISTILL, bool TOPK, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
   constexpr int N = Elem<T>::N, NW = NT / 32, EPT = kVocabMaxTeacher / NT;  // teacher entries of a thread

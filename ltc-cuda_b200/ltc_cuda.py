@@ -896,7 +896,9 @@ def ltc_linear_scan(a, b, h0=None, seq_starts=None) -> Tuple[torch.Tensor, torch
     same, any batch and time strides.  ``h0`` (fp32 ``(B, H)`` or ``(S, H)``) defaults to
     zeros.  ``h`` has the type of the inputs, ``h_final`` is fp32, and so is the state in
     between.  Tokens that belong to no sequence give 0 and get no gradient; a sequence
-    without tokens returns its ``h0``.  Differentiable once in ``a``, ``b`` and ``h0``."""
+    without tokens returns its ``h0``.  Runs of tokens are folded by their products of ``a``:
+    a product over 128 tokens past fp32's range gives infinities or NaN even where the state
+    is 0 (``|a| <= 1`` is always safe).  Differentiable once in ``a``, ``b`` and ``h0``."""
     tensors, h0, seq_starts, dims = _scan_operands(("a", "b"), (a, b), h0, seq_starts)
     return _scan(None, h0, seq_starts, dims, 0.0, tensors)
 
@@ -1061,7 +1063,8 @@ def ltc_distill_loss(logits, teacher_ids, teacher_logits, temperature: float = 1
     ``teacher_logits`` (logits or log probabilities, any of the three types) ``(..., K)``,
     ``K <= 256``.  A negative id is no entry; a row without entries costs 0 and gets no
     gradient; an id past the vocabulary makes its row NaN.  The gradient goes to ``logits``
-    alone (the teacher is a constant), once, rounded once to their type."""
+    alone (the teacher is a constant), once, rounded once to their type; a row whose loss gets
+    a zero gradient gets zeros, whatever its logits."""
     z, desc = _logits_operand(logits, float(temperature))
     _typed(teacher_logits, "teacher_logits", device=z.device)
     shape = teacher_logits.shape
@@ -1136,8 +1139,8 @@ def ltc_token_logprobs(logits, tokens, top_k: int = 0, temperature: float = 1.0)
     gives NaN.  ``top_ids`` / ``top_logprobs`` ``(..., top_k)`` are sorted, ties to the
     lowest id (``None`` when ``top_k`` is 0); where fewer entries are above ``-inf`` they
     hold -1 and ``-inf``.  A row of nothing but ``-inf`` has log probabilities ``-inf``,
-    entropy 0 and gradient 0.  Differentiable once in ``logits`` through ``logprobs`` and
-    ``entropy``."""
+    entropy 0 and gradient 0; NaN or ``+inf`` in a row makes its scores NaN and its alternatives
+    unspecified ids.  Differentiable once in ``logits`` through ``logprobs`` and ``entropy``."""
     z, desc = _logits_operand(logits, float(temperature))
     tok = _id_operand(tokens, "tokens", z.device, z.shape[:-1])
     top_k = int(top_k)
