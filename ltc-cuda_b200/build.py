@@ -2,7 +2,8 @@
 
 Usage: python build.py [--verbose-ptxas]
 The library is written next to this file (``libltc_sm100.so``); it has no
-torch dependency (plain C-ABI over the CUDA runtime).
+torch dependency (plain C-ABI over the CUDA runtime).  ``ltc_torch.so`` beside it is the
+torch binding of the sequence operators, host code only.
 """
 from __future__ import annotations
 
@@ -17,6 +18,7 @@ import tempfile
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libltc_sm100.so")
+TORCH_BINDING = os.path.join(HERE, "ltc_torch.so")
 SOURCES = ["ltc_capi.cu", "ltc_prep.cu", "ltc_sensory.cu", "ltc_recurrent.cu", "ltc_recurrent_wide.cu",
            "ltc_noalloc.cu", "ltc_recurrent_stream.cu", "ltc_recurrent_sparse.cu", "ltc_recurrent_csparse.cu",
            "ltc_preamble.cu", "ltc_sensory_sparse.cu", "ltc_scan.cu", "ltc_vocab.cu"]
@@ -70,6 +72,26 @@ def build(force: bool = False, verbose_ptxas: bool = False, out: str = LIB, defi
     return out
 
 
+def build_torch_binding() -> str:
+    """g++ csrc/ltc_torch.cpp against the torch that runs this."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in include],
+           "-o", TORCH_BINDING + ".tmp", os.path.join(CSRC, "ltc_torch.cpp"), f"-L{os.path.join(root, 'lib')}",
+           "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed building ltc_torch.so")
+    os.replace(TORCH_BINDING + ".tmp", TORCH_BINDING)
+    return TORCH_BINDING
+
+
 if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("--verbose-ptxas", action="store_true")
@@ -81,5 +103,6 @@ if __name__ == "__main__":
     a = ap.parse_args()
     print(build(force=a.force or a.verbose_ptxas, verbose_ptxas=a.verbose_ptxas, out=os.path.abspath(a.out),
                 defines=a.defines))
+    print(build_torch_binding())
     if a.checked:
         print(build(force=True, out=os.path.join(HERE, "libltc_sm100_checked.so"), defines=["LTC_CHECKED"]))

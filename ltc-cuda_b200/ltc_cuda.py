@@ -32,14 +32,13 @@ kernels raises ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
-import functools
+import importlib.util
 import logging
 import os
 import threading
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 logger = logging.getLogger(__name__)
 
@@ -172,6 +171,19 @@ if _lib is None and torch.cuda.is_available():
 
 _HAS_CUDA_KERNELS: bool = _lib is not None and torch.cuda.is_available()
 
+# the sequence operators' torch binding (csrc/ltc_torch.cpp), bound to the library loaded above;
+# the solver does without
+_torch_binding = None
+_binding_error: Optional[str] = None
+try:
+    _spec = importlib.util.spec_from_file_location("ltc_torch", os.path.join(_HERE, "ltc_torch.so"))
+    _torch_binding = importlib.util.module_from_spec(_spec)
+    _spec.loader.exec_module(_torch_binding)
+    if _lib is not None:
+        _torch_binding.bind({n: ctypes.cast(getattr(_lib, n), ctypes.c_void_p).value for n in EXPORTS})
+except ImportError as exc:  # not built, or built against another torch
+    _torch_binding, _binding_error = None, str(exc)
+
 
 def _check(status: int, what: str) -> None:
     if status != 0:
@@ -184,6 +196,14 @@ def _require_kernels() -> ctypes.CDLL:
         raise RuntimeError("ltc_cuda: CUDA kernels unavailable "
                            f"(library: {_load_error or 'loaded'}, cuda: {torch.cuda.is_available()})")
     return _lib
+
+
+def _require_binding():
+    _require_kernels()
+    if _torch_binding is None:
+        raise RuntimeError(f"ltc_cuda: ltc_torch.so could not be loaded ({_binding_error}); "
+                           "build it with `python ltc-cuda_b200/build.py`")
+    return _torch_binding
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -372,6 +392,8 @@ def set_check_waits(on: bool) -> None:
     step boundary they already synchronise on."""
     _CHECK_WAITS[0] = bool(on)
     _CHECK_WAITS[1] = wait_timeouts() if on else 0
+    if _torch_binding is not None:
+        _torch_binding.set_check_waits(_check_waits_after if on else None)
 
 
 def _check_waits_after(where: str) -> None:
@@ -708,49 +730,6 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _scan_input(t: torch.Tensor) -> LtcScanInput:
-    """(B,T,H), (T,H) packed or (B,H) single tokens."""
-    if t.dim() == 3:
-        return LtcScanInput(t.data_ptr(), t.stride(0), t.stride(1))
-    return LtcScanInput(t.data_ptr(), t.stride(0), t.stride(0))
-
-
-def _fresh(t: torch.Tensor) -> torch.Tensor:
-    """A contiguous tensor of t's shape, type and place (``empty_like`` is the cheaper call)."""
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
-
-
-def _current_stream(dev) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)
-
-
-class _OnDevice:
-    """``torch.cuda.device`` for the common case that the device is the current one already."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, dev):
-        self.guard = None if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
-
-
-@functools.lru_cache(maxsize=1024)
-def _scan_plan(index: int, dims: Tuple[int, int, int, int], dtype: int) -> Tuple[int, int, int]:
-    """(saved, forward workspace, backward workspace) bytes on the current device, number ``index``."""
-    p = LtcScanPlan()
-    B, T, H, S = dims
-    _check(_lib.ltc_scan_plan(ctypes.byref(LtcScanDims(B, T, H, dtype, S)), ctypes.byref(p)), "ltc_scan_plan")
-    return p.saved_bytes, p.fwd_workspace_bytes, p.bwd_workspace_bytes
-
-
 def _alike(t, name: str, first: torch.Tensor) -> None:
     """``t`` has the type, place and shape of ``first``."""
     if not (isinstance(t, torch.Tensor) and t.dtype is first.dtype and t.device == first.device):
@@ -800,92 +779,8 @@ def _check_decay(decay, device, H: int, scale: float) -> torch.Tensor:
     return decay
 
 
-def _scan_forward(decay, h0, seq_starts, dims, scale, keep, inputs):
-    """(h, h_final, what a backward needs besides the operands; ``keep``: one follows)."""
-    lib = _require_kernels()
-    B, T, H, S = dims
-    first = inputs[0]
-    dev, dtype = first.device, first.dtype
-    h = _fresh(first)
-    h_final = torch.empty(S or B, H, device=dev, dtype=torch.float32) if h0 is None else torch.empty_like(h0)
-    if first.numel() == 0:
-        h_final.zero_() if h0 is None else h_final.copy_(h0)
-        return h, h_final, None
-    code = _DTYPES[dtype]
-    with _OnDevice(dev):
-        saved_bytes, ws_bytes, _ = _scan_plan(dev.index, dims, code)
-        saved = torch.empty(saved_bytes, device=dev, dtype=torch.uint8) if keep and saved_bytes else None
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
-        ins = [ctypes.byref(_scan_input(t)) for t in inputs]
-        tail = (_ptr(h0), _ptr(seq_starts), h.data_ptr(), h_final.data_ptr(), _ptr(saved), _ptr(ws), ws_bytes,
-                _current_stream(dev))
-        cd = ctypes.byref(LtcScanDims(B, T, H, code, S))
-        if decay is None:
-            _check(lib.ltc_linear_scan_forward(cd, *ins, *tail), "ltc_linear_scan")
-        else:
-            _check(lib.ltc_gated_scan_forward(cd, *ins, decay.data_ptr(), scale, *tail), "ltc_gated_scan")
-    return h, h_final, saved
-
-
-class _ScanFunction(torch.autograd.Function):
-    """Both scans: ``inputs`` are (a, b), or (x, rate, gate) with ``decay``."""
-
-    @staticmethod
-    def forward(ctx, decay, h0, seq_starts, dims, scale, *inputs):
-        h, h_final, saved = _scan_forward(decay, h0, seq_starts, dims, scale, True, inputs)
-        ctx.dims, ctx.scale = dims, scale
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(decay, h0, seq_starts, saved, *inputs)
-        return h, h_final
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh, dh_final):
-        lib = _require_kernels()
-        decay, h0, seq_starts, saved, *inputs = ctx.saved_tensors
-        B, T, H, S = ctx.dims
-        first = inputs[0]
-        dev = first.device
-        grads = [_fresh(t) for t in inputs]
-        dh0 = None if h0 is None else torch.empty_like(h0)
-        ddecay = None if decay is None else torch.empty_like(decay)
-        if first.numel() == 0:
-            if dh0 is not None:
-                dh0.zero_() if dh_final is None else dh0.copy_(dh_final)
-            if ddecay is not None:
-                ddecay.zero_()
-            return (ddecay, dh0, None, None, None, *grads)
-        if dh is not None:
-            dh = _rows(dh.to(first.dtype))
-            dh = dh if dh.stride(-2) <= SCAN_MAX_H else dh.contiguous()
-        if dh_final is not None:
-            dh_final = dh_final.to(torch.float32).contiguous()
-        cd = LtcScanDims(B, T, H, _DTYPES[first.dtype], S)
-        ins = [ctypes.byref(_scan_input(t)) for t in inputs]
-        with _OnDevice(dev):
-            _, _, ws_bytes = _scan_plan(dev.index, ctx.dims, cd.dtype)
-            ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-            mid = (_ptr(h0), _ptr(seq_starts), _ptr(saved), None if dh is None else ctypes.byref(_scan_input(dh)),
-                   _ptr(dh_final), *[g.data_ptr() for g in grads])
-            tail = (_ptr(dh0), ws.data_ptr(), ws_bytes, _current_stream(dev))
-            if decay is None:
-                _check(lib.ltc_linear_scan_backward(ctypes.byref(cd), *ins, *mid, *tail), "ltc_linear_scan backward")
-            else:
-                _check(lib.ltc_gated_scan_backward(ctypes.byref(cd), *ins, decay.data_ptr(), ctx.scale, *mid,
-                                                   ddecay.data_ptr(), *tail), "ltc_gated_scan backward")
-        if _CHECK_WAITS[0]:
-            _check_waits_after("scan backward")
-        return (ddecay, dh0, None, None, None, *grads)
-
-
 def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _scan(decay, h0, seq_starts, dims, scale, inputs):
-    if _wants_grad(*inputs, decay, h0):
-        return _ScanFunction.apply(decay, h0, seq_starts, dims, scale, *inputs)
-    return _scan_forward(decay, h0, seq_starts, dims, scale, False, inputs)[:2]
 
 
 def ltc_linear_scan(a, b, h0=None, seq_starts=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -900,7 +795,7 @@ def ltc_linear_scan(a, b, h0=None, seq_starts=None) -> Tuple[torch.Tensor, torch
     a product over 128 tokens past fp32's range gives infinities or NaN even where the state
     is 0 (``|a| <= 1`` is always safe).  Differentiable once in ``a``, ``b`` and ``h0``."""
     tensors, h0, seq_starts, dims = _scan_operands(("a", "b"), (a, b), h0, seq_starts)
-    return _scan(None, h0, seq_starts, dims, 0.0, tensors)
+    return _require_binding().scan(None, h0, seq_starts, dims, 0.0, tensors)
 
 
 def ltc_gated_scan(x, rate, gate, decay, h0=None, seq_starts=None, scale: float = 8.0):
@@ -914,7 +809,7 @@ def ltc_gated_scan(x, rate, gate, decay, h0=None, seq_starts=None, scale: float 
     inside the scan.  Differentiable once in all of them and ``h0``."""
     tensors, h0, seq_starts, dims = _scan_operands(("x", "rate", "gate"), (x, rate, gate), h0, seq_starts)
     decay = _check_decay(decay, tensors[0].device, dims[2], scale)
-    return _scan(decay, h0, seq_starts, dims, float(scale), tensors)
+    return _require_binding().scan(decay, h0, seq_starts, dims, float(scale), tensors)
 
 
 def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_state=None):
@@ -935,23 +830,13 @@ def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_sta
         raise ValueError(f"state has shape {tuple(s.shape)}, expected {tuple(first.shape)}")
     if _wants_grad(x, rate, gate, decay, state):
         raise RuntimeError("ltc_gated_scan_step has no backward pass; use ltc_gated_scan or torch.no_grad()")
-    if out_state is None:
-        out_state = torch.empty_like(s)
-    elif (not isinstance(out_state, torch.Tensor) or out_state.dtype != torch.float32 or out_state.device != dev
-          or out_state.shape != first.shape or not out_state.is_contiguous()):
-        raise ValueError("out_state must be a contiguous fp32 tensor shaped and placed like x")
-    elif 0 < abs(out_state.data_ptr() - s.data_ptr()) < 4 * s.numel():
-        raise ValueError("out_state may be state itself but not overlap it otherwise")
-    lib = _require_kernels()
-    h = _fresh(first)
-    if h.numel():
-        cd = LtcScanDims(B, 1, H, _DTYPES[first.dtype], 0)
-        ins = [ctypes.byref(_scan_input(_rows(t))) for t in (x, rate, gate)]
-        with _OnDevice(dev):
-            _check(lib.ltc_gated_scan_step(ctypes.byref(cd), *ins, decay.data_ptr(), float(scale), s.data_ptr(),
-                                           h.data_ptr(), out_state.data_ptr(), _current_stream(dev)),
-                   "ltc_gated_scan_step")
-    return h, out_state
+    if out_state is not None:
+        if (not isinstance(out_state, torch.Tensor) or out_state.dtype != torch.float32 or out_state.device != dev
+                or out_state.shape != first.shape or not out_state.is_contiguous()):
+            raise ValueError("out_state must be a contiguous fp32 tensor shaped and placed like x")
+        if 0 < abs(out_state.data_ptr() - s.data_ptr()) < 4 * s.numel():
+            raise ValueError("out_state may be state itself but not overlap it otherwise")
+    return _require_binding().gated_step(_rows(x), _rows(rate), _rows(gate), decay, s, out_state, float(scale))
 
 
 # ---------------------------------------------------------------------------
@@ -1003,55 +888,6 @@ def _id_operand(t, name: str, device, shape) -> torch.Tensor:
     return t.to(torch.int64).contiguous()
 
 
-def _row_grad(g: Optional[torch.Tensor], rows: int):
-    """(tensor, stride) of a per-row gradient; one that is the same for all rows stays a single value."""
-    if g is None:
-        return None, 0
-    g = g.to(torch.float32)
-    if rows > 1 and all(st == 0 or n == 1 for n, st in zip(g.shape, g.stride())):
-        return g, 0
-    return g.contiguous(), 1
-
-
-def _distill_forward(z, ids, teacher, desc, keep):
-    """(loss, teacher probabilities and row statistics for a backward)"""
-    lib = _require_kernels()
-    dev, rows, K = z.device, desc[0], ids.shape[-1]
-    loss = torch.empty(z.shape[:-1], device=dev, dtype=torch.float32)
-    probs = torch.empty(rows, K, device=dev, dtype=torch.float32) if keep else None
-    stats = torch.empty(rows, 4, device=dev, dtype=torch.float32) if keep else None
-    if rows:
-        with _OnDevice(dev):
-            _check(lib.ltc_distill_forward(ctypes.byref(LtcLogits(z.data_ptr(), *desc)), ids.data_ptr(),
-                                           teacher.data_ptr(), _DTYPES[teacher.dtype], K, loss.data_ptr(),
-                                           _ptr(probs), _ptr(stats), _current_stream(dev)), "ltc_distill_loss")
-    return loss, probs, stats
-
-
-class _DistillLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, ids, teacher, desc):
-        loss, probs, stats = _distill_forward(z, ids, teacher, desc, True)
-        ctx.desc = desc
-        ctx.save_for_backward(z, ids, probs, stats)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        lib = _require_kernels()
-        z, ids, probs, stats = ctx.saved_tensors
-        dz = _fresh(z)
-        g, stride = _row_grad(g, ctx.desc[0])
-        if ctx.desc[0]:
-            with _OnDevice(z.device):
-                _check(lib.ltc_distill_backward(ctypes.byref(LtcLogits(z.data_ptr(), *ctx.desc)), ids.data_ptr(),
-                                                ids.shape[-1], probs.data_ptr(), stats.data_ptr(), g.data_ptr(),
-                                                stride, dz.data_ptr(), _current_stream(z.device)),
-                       "ltc_distill_loss backward")
-        return dz, None, None, None
-
-
 def ltc_distill_loss(logits, teacher_ids, teacher_logits, temperature: float = 1.0) -> torch.Tensor:
     """Distillation from a teacher's top entries -> fp32 losses ``logits.shape[:-1]``:
 
@@ -1073,8 +909,7 @@ def ltc_distill_loss(logits, teacher_ids, teacher_logits, temperature: float = 1
                          f"with 1 <= K <= {DISTILL_MAX_K}")
     ids = _id_operand(teacher_ids, "teacher_ids", z.device, shape)
     teacher = teacher_logits.detach().contiguous()
-    return _DistillLoss.apply(z, ids, teacher, desc) if _wants_grad(z) else _distill_forward(z, ids, teacher, desc,
-                                                                                             False)[0]
+    return _require_binding().distill(z, ids, teacher, desc[:4], desc[6])
 
 
 class TokenLogprobs(NamedTuple):
@@ -1082,52 +917,6 @@ class TokenLogprobs(NamedTuple):
     entropy: torch.Tensor
     top_ids: Optional[torch.Tensor]
     top_logprobs: Optional[torch.Tensor]
-
-
-def _token_logprobs_forward(z, tokens, desc, top_k, keep):
-    """(log probabilities, entropies, top ids and log probabilities, row statistics for a backward)"""
-    lib = _require_kernels()
-    dev, rows, lead = z.device, desc[0], z.shape[:-1]
-    lp = torch.empty(lead, device=dev, dtype=torch.float32)
-    ent = torch.empty(lead, device=dev, dtype=torch.float32)
-    stats = torch.empty(rows, 4, device=dev, dtype=torch.float32) if keep else None
-    top_ids = torch.empty(*lead, top_k, device=dev, dtype=torch.int64) if top_k else None
-    top_lp = torch.empty(*lead, top_k, device=dev, dtype=torch.float32) if top_k else None
-    if rows:
-        with _OnDevice(dev):
-            _check(lib.ltc_token_logprobs_forward(ctypes.byref(LtcLogits(z.data_ptr(), *desc)), tokens.data_ptr(),
-                                                  top_k, lp.data_ptr(), ent.data_ptr(), _ptr(top_ids), _ptr(top_lp),
-                                                  _ptr(stats), _current_stream(dev)), "ltc_token_logprobs")
-    return lp, ent, top_ids, top_lp, stats
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, tokens, desc, top_k):
-        lp, ent, top_ids, top_lp, stats = _token_logprobs_forward(z, tokens, desc, top_k, True)
-        ctx.desc = desc
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(z, tokens, stats)
-        if top_k:
-            ctx.mark_non_differentiable(top_ids, top_lp)
-        return lp, ent, top_ids, top_lp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_ent, *_):
-        lib = _require_kernels()
-        z, tokens, stats = ctx.saved_tensors
-        rows = ctx.desc[0]
-        dz = _fresh(z)
-        g_lp, lp_stride = _row_grad(g_lp, rows)
-        g_ent, ent_stride = _row_grad(g_ent, rows)
-        if rows:
-            with _OnDevice(z.device):
-                _check(lib.ltc_token_logprobs_backward(ctypes.byref(LtcLogits(z.data_ptr(), *ctx.desc)),
-                                                       tokens.data_ptr(), stats.data_ptr(), _ptr(g_lp), lp_stride,
-                                                       _ptr(g_ent), ent_stride, dz.data_ptr(),
-                                                       _current_stream(z.device)), "ltc_token_logprobs backward")
-        return dz, None, None, None
 
 
 def ltc_token_logprobs(logits, tokens, top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
@@ -1146,6 +935,4 @@ def ltc_token_logprobs(logits, tokens, top_k: int = 0, temperature: float = 1.0)
     top_k = int(top_k)
     if not 0 <= top_k <= min(TOKEN_LOGPROBS_MAX_TOP, z.shape[-1]):
         raise ValueError(f"top_k must be between 0 and min({TOKEN_LOGPROBS_MAX_TOP}, V) (got {top_k})")
-    if _wants_grad(z):
-        return TokenLogprobs(*_TokenLogprobs.apply(z, tok, desc, top_k))
-    return TokenLogprobs(*_token_logprobs_forward(z, tok, desc, top_k, False)[:4])
+    return TokenLogprobs(*_require_binding().scores(z, tok, desc[:4], desc[6], top_k))

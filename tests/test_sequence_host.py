@@ -174,3 +174,16 @@ def test_two_ranks_train_and_score_like_one(monkeypatch):
     assert torch.allclose(torch.tensor(g2), grad, rtol=1e-5, atol=1e-6)
     assert torch.allclose(torch.tensor(s2, dtype=torch.float64), sums, rtol=1e-5)
     assert sums[2] == (_data()[3] >= 0).sum()
+
+
+def test_missing_binding_is_named(monkeypatch):
+    """The solver works without ltc_torch.so; the sequence operators say that it is missing."""
+    monkeypatch.setattr(ltc_cuda, "_HAS_CUDA_KERNELS", True)
+    monkeypatch.setattr(ltc_cuda, "_torch_binding", None)
+    monkeypatch.setattr(ltc_cuda, "_on_cuda", lambda t, name: None)
+    for call in (lambda: ltc_cuda.ltc_linear_scan(t(1, 2, 3), t(1, 2, 3)),
+                 lambda: ltc_cuda.ltc_gated_scan_step(t(2, 3), t(2, 3), t(2, 3), t(3), t(2, 3)),
+                 lambda: ltc_cuda.ltc_distill_loss(t(2, 9), torch.zeros(2, 4, dtype=torch.long), t(2, 4)),
+                 lambda: ltc_cuda.ltc_token_logprobs(t(2, 9), torch.zeros(2, dtype=torch.long))):
+        with pytest.raises(RuntimeError, match="ltc_torch.so could not be loaded"):
+            call()
