@@ -704,6 +704,7 @@ def ltc_preamble(x, ln_w, ln_b, in_w, in_b, eps: float):
 # ---------------------------------------------------------------------------
 SCAN_MAX_H = 1 << 28
 SCAN_MAX_T = 0x7fff0000
+SCAN_MAX_B = 0x7fffffff
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -738,6 +739,11 @@ def _alike(t, name: str, first: torch.Tensor) -> None:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(first.shape)}")
 
 
+def _check_batch(n: int) -> None:
+    if n > SCAN_MAX_B:
+        raise ValueError(f"more than 2^31 - 1 sequences (got {n})")
+
+
 def _scan_operands(names, tensors, h0, seq_starts):
     """Checked operands of a scan: (inputs, h0, seq_starts, dims as (B, T, H, S))."""
     first = _typed(tensors[0], names[0])
@@ -759,7 +765,7 @@ def _scan_operands(names, tensors, h0, seq_starts):
             raise ValueError(f"seq_starts is on {seq_starts.device}, expected {first.device}")
         T, H = first.shape
         B, S = 1, seq_starts.numel() - 1
-        seq_starts = seq_starts.to(torch.int32).contiguous()
+    _check_batch(S or B)
     if T > SCAN_MAX_T or H > SCAN_MAX_H or any(t.stride(-2) > SCAN_MAX_H for t in tensors):
         raise ValueError("more than 2^31 - 2^16 time steps, 2^28 channels, or a time stride past 2^28 elements")
     if h0 is not None:
@@ -767,6 +773,8 @@ def _scan_operands(names, tensors, h0, seq_starts):
         if h0.shape != (S or B, H):
             raise ValueError(f"h0 has shape {tuple(h0.shape)}, expected {(S or B, H)}")
     _on_cuda(first, names[0])
+    if seq_starts is not None:
+        seq_starts = seq_starts.to(torch.int32).contiguous()
     return [_rows(t) for t in tensors], h0, seq_starts, (B, T, H, S)
 
 
@@ -823,6 +831,9 @@ def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_sta
     dev, (B, H) = first.device, first.shape
     _alike(rate, "rate", first)
     _alike(gate, "gate", first)
+    _check_batch(B)
+    if H > SCAN_MAX_H:
+        raise ValueError("more than 2^28 channels")
     _on_cuda(first, "x")
     decay = _check_decay(decay, dev, H, scale)
     s = _as_f32(state, dev, "state")

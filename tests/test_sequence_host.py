@@ -187,3 +187,17 @@ def test_missing_binding_is_named(monkeypatch):
                  lambda: ltc_cuda.ltc_token_logprobs(t(2, 9), torch.zeros(2, dtype=torch.long))):
         with pytest.raises(RuntimeError, match="ltc_torch.so could not be loaded"):
             call()
+
+
+def test_batch_past_31_bits_is_refused():
+    """One more than the kernels' 31-bit count of sequences, and one that wraps to a small number."""
+    for n in (1 << 31, (1 << 32) + 5):
+        wide = t(1, 1, 1).expand(n, 1, 1)
+        with pytest.raises(ValueError, match="sequences"):
+            ltc_cuda.ltc_linear_scan(wide, wide)
+        rows = t(1, 1).expand(n, 1)
+        with pytest.raises(ValueError, match="sequences"):
+            ltc_cuda.ltc_gated_scan_step(rows, rows, rows, t(1), rows)
+        starts = torch.zeros(1, dtype=torch.int32).expand(n + 1)
+        with pytest.raises(ValueError, match="sequences"):
+            ltc_cuda.ltc_gated_scan(t(4, 3), t(4, 3), t(4, 3), t(3), seq_starts=starts)
