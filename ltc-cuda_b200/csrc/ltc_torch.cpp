@@ -10,9 +10,11 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <atomic>
+#include <cmath>
 
 #include "../../include/ltc_sm100.h"
 
@@ -244,17 +246,56 @@ std::pair<Tensor, Tensor> scan(const OptTensor& decay_, const OptTensor& h0_, co
   return {r[0], r[1]};
 }
 
-std::pair<Tensor, Tensor> gated_step(const Tensor& x, const Tensor& rate, const Tensor& gate, const Tensor& decay,
-                                     const Tensor& state, const OptTensor& out_, double scale) {
-  const Tensor h = fresh(x), out = out_.has_value() ? *out_ : floats(x, x.sizes());
-  if (h.numel()) {
-    const c10::cuda::CUDAGuard guard(x.device());
-    const LtcScanDims d{static_cast<int32_t>(x.size(0)), 1, static_cast<int32_t>(x.size(1)), dtype_of(x), 0};
-    const LtcScanInput a = input_of(x), b = input_of(rate), c = input_of(gate);
-    check(lib.ltc_gated_scan_step(&d, &a, &b, &c, ptr(decay), static_cast<float>(scale), ptr(state), h.data_ptr(),
-                                  ptr(out), stream_of(x)), "ltc_gated_scan_step");
+bool is_floats(const Tensor& t, const Tensor& like, at::IntArrayRef shape) {
+  return t.scalar_type() == at::kFloat && t.device() == like.device() && t.sizes() == shape && t.is_contiguous();
+}
+
+// The one-token step: (h, new state), or None for operands that ltc_cuda.py has to look at (to
+// copy them, or to name what is wrong).  Its checks are these in Python, where they took half of
+// a call; so they come first here and only what fails them goes through Python's.
+py::object gated_step(py::handle x_, py::handle rate_, py::handle gate_, py::handle decay_, py::handle state_,
+                      py::handle out_, py::handle scale_) {
+  for (const py::handle& o : {x_, rate_, gate_, decay_, state_})
+    if (!THPVariable_Check(o.ptr())) return py::none();
+  const bool given = !out_.is_none();
+  if ((given && !THPVariable_Check(out_.ptr())) || !PyFloat_Check(scale_.ptr())) return py::none();
+  const double scale = PyFloat_AS_DOUBLE(scale_.ptr());
+  if (!(scale > 0.0) || std::isinf(scale)) return py::none();
+  const Tensor &x = THPVariable_Unpack(x_.ptr()), &rate = THPVariable_Unpack(rate_.ptr()),
+               &gate = THPVariable_Unpack(gate_.ptr()), &decay = THPVariable_Unpack(decay_.ptr()),
+               &state = THPVariable_Unpack(state_.ptr());
+  const auto type = x.scalar_type();
+  if (x.dim() != 2 || !x.is_cuda() || (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf))
+    return py::none();
+  const int64_t B = x.size(0), H = x.size(1);
+  if (B > INT32_MAX || H > (1 << 28)) return py::none();
+  for (const Tensor* t : {&x, &rate, &gate})
+    if (t->scalar_type() != type || t->device() != x.device() || t->sizes() != x.sizes() ||
+        (t->stride(1) != 1 && H != 1))
+      return py::none();
+  if (!is_floats(decay, x, {H}) || !is_floats(state, x, x.sizes())) return py::none();
+  if (wants_grad({x, rate, gate, decay, state})) return py::none();
+  Tensor out;
+  if (given) {
+    out = THPVariable_Unpack(out_.ptr());
+    if (!is_floats(out, x, x.sizes())) return py::none();
+    const intptr_t apart = static_cast<char*>(out.data_ptr()) - static_cast<char*>(state.data_ptr());
+    if (apart != 0 && std::abs(apart) < 4 * state.numel()) return py::none();
   }
-  return {h, out};
+  Tensor h;
+  {
+    const py::gil_scoped_release release;
+    h = fresh(x);
+    if (!given) out = floats(x, x.sizes());
+    if (h.numel()) {
+      const c10::cuda::CUDAGuard guard(x.device());
+      const LtcScanDims d{static_cast<int32_t>(B), 1, static_cast<int32_t>(H), dtype_of(x), 0};
+      const LtcScanInput a = input_of(x), b = input_of(rate), c = input_of(gate);
+      check(lib.ltc_gated_scan_step(&d, &a, &b, &c, ptr(decay), static_cast<float>(scale), ptr(state), h.data_ptr(),
+                                    ptr(out), stream_of(x)), "ltc_gated_scan_step");
+    }
+  }
+  return py::make_tuple(h, out);
 }
 
 // ---- vocabulary --------------------------------------------------------------------
@@ -418,7 +459,7 @@ PYBIND11_MODULE(ltc_torch, m) {
   // the interpreter is free while a call allocates and launches
   const auto release = py::call_guard<py::gil_scoped_release>();
   m.def("scan", &scan, release);
-  m.def("gated_step", &gated_step, release);
+  m.def("gated_step", &gated_step);
   m.def("distill", &distill, release);
   m.def("scores", &scores, release);
 }

@@ -825,6 +825,11 @@ def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_sta
     ``(B, H)`` -> ``(h, new_state)``, what :func:`ltc_gated_scan` gives for ``T = 1``.
     ``out_state`` receives the new state; ``out_state=state`` updates it in place.  Not
     differentiable: raises where a gradient would be recorded."""
+    if _torch_binding is not None:
+        done = _torch_binding.gated_step(x, rate, gate, decay, state, out_state, scale)
+        if done is not None:
+            return done
+    # something to copy, or to refuse
     first = _typed(x, "x")
     if first.dim() != 2:
         raise ValueError(f"x must be (B, H), got shape {tuple(first.shape)}")
@@ -847,7 +852,10 @@ def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_sta
             raise ValueError("out_state must be a contiguous fp32 tensor shaped and placed like x")
         if 0 < abs(out_state.data_ptr() - s.data_ptr()) < 4 * s.numel():
             raise ValueError("out_state may be state itself but not overlap it otherwise")
-    return _require_binding().gated_step(_rows(x), _rows(rate), _rows(gate), decay, s, out_state, float(scale))
+    done = _require_binding().gated_step(_rows(x), _rows(rate), _rows(gate), decay, s, out_state, float(scale))
+    if done is None:
+        raise RuntimeError("ltc_cuda.ltc_gated_scan_step: the binding refused checked operands")
+    return done
 
 
 # ---------------------------------------------------------------------------

@@ -137,3 +137,43 @@ def test_wait_check(monkeypatch):
         monkeypatch.undo()
         ltc_cuda.set_check_waits(False)
     ltc_cuda.ltc_gated_scan(x, rate, gate, decay)[0].sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_step_operands_that_need_a_copy(dtype):
+    """Ordinary operands go straight to the binding; the others give the same through a copy."""
+    g = torch.Generator().manual_seed(3)
+    x, rate, gate = (torch.randn(5, 12, generator=g).to(dtype).cuda() for _ in range(3))
+    decay, state = torch.randn(12, generator=g).cuda(), torch.randn(5, 12, generator=g).cuda()
+    want = ltc_cuda.ltc_gated_scan_step(x, rate, gate, decay, state)
+    turned = lambda t: t.t().contiguous().t()  # noqa: E731
+    spread = torch.stack([decay, decay], 1)[:, 0]
+    assert turned(x).stride(-1) != 1 and spread.stride(0) == 2
+    for args in ((turned(x), rate, gate, decay, state), (x, rate, turned(gate), decay, state),
+                 (x, rate, gate, spread, state), (x, rate, gate, decay, turned(state))):
+        assert all(torch.equal(u, v) for u, v in zip(ltc_cuda.ltc_gated_scan_step(*args), want))
+    for scale in (8, torch.tensor(8.0).item()):
+        got = ltc_cuda.ltc_gated_scan_step(x, rate, gate, decay, state, scale=scale)
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+def test_step_refusals_on_the_gpu():
+    z = torch.zeros(4, 6, device="cuda")
+    d = torch.zeros(6, device="cuda")
+    pool = torch.zeros(30, device="cuda")
+    step = ltc_cuda.ltc_gated_scan_step
+    for exc, args, kw in (
+            (TypeError, (z.double(), z, z, d, z), {}), (TypeError, (z, z.bfloat16(), z, d, z), {}),
+            (TypeError, (z, z, z, d.half(), z), {}), (ValueError, (z, z[:2], z, d, z), {}),
+            (ValueError, (z, z, z, d[:5], z), {}), (ValueError, (z, z, z, d, z.cpu()), {}),
+            (ValueError, (z, z, z, d, z[:, :5]), {}), (ValueError, (z, z, z, d, z), dict(scale=0.0)),
+            (ValueError, (z, z, z, d, z), dict(scale=float("nan"))),
+            (ValueError, (z, z, z, d, z), dict(scale=float("inf"))),
+            (ValueError, (z, z, z, d, z), dict(out_state=z.half())),
+            (ValueError, (z, z, z, d, z), dict(out_state=torch.zeros(6, 4, device="cuda").t())),
+            (ValueError, (z, z, z, d, pool[:24].view(4, 6)), dict(out_state=pool[6:].view(4, 6))),
+            (RuntimeError, (z, z, z, d.clone().requires_grad_(), z), {}),
+            (TypeError, ([1.0], z, z, d, z), {})):
+        with pytest.raises(exc):
+            step(*args, **kw)
+    assert step(z, z, z, d, z)[0].shape == (4, 6)
