@@ -15,7 +15,6 @@ Definitions (all per channel h; t runs inside one sequence):
                 loss = tau^2 * sum_k p_k (log p_k - log q_{id_k})
   token scores  q as above; log q[token], entropy -sum q log q, the top-k entries of log q
 """
-import functools
 import math
 import os
 import sys
@@ -29,9 +28,7 @@ _BYTES = {"fp32": 4, "bf16": 2, "fp16": 2}
 _SCALE = 8.0
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
-    """The package, imported once as a user's program does."""
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     path = os.path.join(root, "ltc-cuda_b200")
     if path not in sys.path:
