@@ -99,6 +99,17 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     if (t.defined() && t.requires_grad()) return true;
   return false;
 }
+// Saved tensors come back as a saved-tensor hook left them (offloaded, repacked): the values are the
+// forward's, the layout need not be.  `t` as a contiguous array of the forward's type and length.
+Tensor restored(const Tensor& t, at::ScalarType type, int64_t n, const at::Device& on) {
+  if (!t.defined()) return t;
+  TORCH_CHECK(t.scalar_type() == type && t.numel() == n && t.device() == on,
+              "ltc_cuda: a saved tensor came back as ", t.numel(), " x ", t.scalar_type(), " on ", t.device(),
+              ", saved as ", n, " x ", type, " on ", on);
+  const Tensor c = t.contiguous();
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(c.data_ptr()) % 4 == 0, "ltc_cuda: a saved tensor came back misaligned");
+  return c;
+}
 // Gradients of a backward that is itself recorded: the first order stands, and the second raises.
 // The raising node hangs on the operator's own inputs, so every path back to them meets it.
 variable_list once(variable_list grads, variable_list inputs) {
@@ -126,6 +137,16 @@ struct Scan {
 
 LtcScanInput input_of(const Tensor& t) {
   return {t.data_ptr(), t.stride(0), t.dim() == 3 ? t.stride(1) : t.stride(0)};
+}
+
+// A saved scan input: the forward's type and shape, channels contiguous and time strides in range, as
+// the forward's checks had them.
+Tensor restored_rows(const Tensor& t, const LtcScanDims& d, const at::Device& on) {
+  const bool packed = d.num_seqs > 0;
+  TORCH_CHECK(t.defined() && t.is_cuda() && dtype_of(t) == d.dtype && t.device() == on && t.dim() == (packed ? 2 : 3) &&
+                  t.size(-1) == d.H && t.size(-2) == d.T && (packed || t.size(0) == d.B),
+              "ltc_cuda: a saved scan input came back with another type, shape or device");
+  return (t.stride(-1) != 1 && d.H != 1) || t.stride(-2) > (1 << 28) ? t.contiguous() : t;
 }
 
 // (h, h_final, saved)
@@ -179,15 +200,21 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
       const at::NoGradGuard no_grad;
       const auto v = ctx->get_saved_variables();
       inputs = {v[0], v[1], v[4], v[5], v[6]};
-      const Tensor &decay = v[0], &h0 = v[1], &starts = v[2], &saved = v[3], &first = v[4];
       const auto n = ctx->saved_data["dims"].toIntVector();
       const LtcScanDims d{static_cast<int32_t>(n[0]), static_cast<int32_t>(n[1]), static_cast<int32_t>(n[2]),
                           static_cast<int32_t>(n[3]), static_cast<int32_t>(n[4])};
       const bool gated = n[5] != 0;
+      Tensor in[3];
+      for (int i = 0; i < (gated ? 3 : 2); ++i) in[i] = restored_rows(v[4 + i], d, v[4].device());
+      const Tensor& first = in[0];
+      const at::Device on = first.device();
+      const Tensor decay = restored(v[0], at::kFloat, d.H, on);
+      const Tensor h0 = restored(v[1], at::kFloat, static_cast<int64_t>(d.num_seqs ? d.num_seqs : d.B) * d.H, on);
+      const Tensor starts = restored(v[2], at::kInt, d.num_seqs + 1, on);
       Tensor dh = g[0], dlast = g[1];
       Tensor ddecay = decay.defined() ? fresh(decay) : Tensor(), dh0 = h0.defined() ? fresh(h0) : Tensor();
       Tensor grads[3];
-      for (int i = 0; i < (gated ? 3 : 2); ++i) grads[i] = fresh(v[4 + i]);
+      for (int i = 0; i < (gated ? 3 : 2); ++i) grads[i] = fresh(in[i]);
       if (first.numel() == 0) {
         if (dh0.defined()) dlast.defined() ? dh0.copy_(dlast) : dh0.zero_();
         if (ddecay.defined()) ddecay.zero_();
@@ -200,13 +227,14 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
         if (dlast.defined()) dlast = dlast.to(at::kFloat).contiguous();
         LtcScanPlan p;
         check(lib.ltc_scan_plan(&d, &p), "ltc_scan_plan");
+        const Tensor saved = restored(v[3], at::kByte, static_cast<int64_t>(p.saved_bytes), on);
         const Tensor ws = bytes(first, p.bwd_workspace_bytes);
-        const LtcScanInput a = input_of(v[4]), b = input_of(v[5]);
+        const LtcScanInput a = input_of(in[0]), b = input_of(in[1]);
         LtcScanInput gh{};
         if (dh.defined()) gh = input_of(dh);
         const LtcScanInput* pgh = dh.defined() ? &gh : nullptr;
         if (gated) {
-          const LtcScanInput c = input_of(v[6]);
+          const LtcScanInput c = input_of(in[2]);
           check(lib.ltc_gated_scan_backward(&d, &a, &b, &c, ptr(decay),
                                             static_cast<float>(ctx->saved_data["scale"].toDouble()), ptr(h0),
                                             ptr<int32_t>(starts), ptr<void>(saved), pgh, ptr(dlast),
@@ -307,13 +335,25 @@ LtcLogits logits_of(const Tensor& z, const Rows& r) {
   return {z.data_ptr(), r.n[0], r.n[1], r.n[2], r.n[3], static_cast<int32_t>(z.size(-1)), dtype_of(z),
           static_cast<float>(r.temperature)};
 }
-void keep_rows(AutogradContext* ctx, const Rows& r) {
-  ctx->saved_data["rows"] = std::vector<int64_t>(r.n.begin(), r.n.end());
+// rows, type, then the sizes and strides that the rows describe
+void keep_rows(AutogradContext* ctx, const Tensor& z, const Rows& r) {
+  std::vector<int64_t> v(r.n.begin(), r.n.end());
+  v.push_back(dtype_of(z));
+  v.insert(v.end(), z.sizes().begin(), z.sizes().end());
+  v.insert(v.end(), z.strides().begin(), z.strides().end());
+  ctx->saved_data["rows"] = std::move(v);
   ctx->saved_data["temperature"] = r.temperature;
 }
-Rows kept_rows(AutogradContext* ctx) {
+// The saved logits and their rows: the recorded ones only for the layout that they were recorded for.
+std::pair<Tensor, Rows> kept_rows(AutogradContext* ctx, const Tensor& z) {
   const auto v = ctx->saved_data["rows"].toIntVector();
-  return {{v[0], v[1], v[2], v[3]}, ctx->saved_data["temperature"].toDouble()};
+  const size_t dims = (v.size() - 5) / 2;
+  const at::IntArrayRef sizes(v.data() + 5, dims), strides(v.data() + 5 + dims, dims);
+  TORCH_CHECK(z.defined() && z.is_cuda() && dtype_of(z) == v[4] && z.sizes() == sizes,
+              "ltc_cuda: the saved logits came back with another type, shape or device");
+  const Rows r{{v[0], v[1], v[2], v[3]}, ctx->saved_data["temperature"].toDouble()};
+  if (z.strides() == strides) return {z, r};
+  return {z.contiguous(), Rows{{v[0], std::max<int64_t>(v[0], 1), 0, sizes.back()}, r.temperature}};
 }
 // a per-row gradient; one that is the same for all rows stays a single value
 std::pair<Tensor, int64_t> row_grad(const Tensor& g, int64_t rows) {
@@ -350,7 +390,7 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [loss, probs, stats] = distill_forward(z, ids, teacher, r, true);
     ctx->save_for_backward({z, ids, probs, stats});
-    keep_rows(ctx, r);
+    keep_rows(ctx, z, r);
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -358,16 +398,19 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
     {
       const at::NoGradGuard no_grad;
       const auto v = ctx->get_saved_variables();
-      const Tensor &z = v[0], &ids = v[1];
-      inputs = {z};
-      const Rows r = kept_rows(ctx);
+      inputs = {v[0]};
+      const auto [z, r] = kept_rows(ctx, v[0]);
+      const int64_t K = v[1].size(-1);
+      const Tensor ids = restored(v[1], at::kLong, r.n[0] * K, z.device());
+      const Tensor probs = restored(v[2], at::kFloat, r.n[0] * K, z.device());
+      const Tensor stats = restored(v[3], at::kFloat, r.n[0] * 4, z.device());
       out[0] = fresh(z);
       if (r.n[0]) {
         const c10::cuda::CUDAGuard guard(z.device());
         const auto [gl, stride] = row_grad(g[0], r.n[0]);
         const LtcLogits l = logits_of(z, r);
-        check(lib.ltc_distill_backward(&l, ptr<int64_t>(ids), static_cast<int32_t>(ids.size(-1)), ptr(v[2]), ptr(v[3]),
-                                       ptr(gl), stride, out[0].data_ptr(), stream_of(z)), "ltc_distill_loss backward");
+        check(lib.ltc_distill_backward(&l, ptr<int64_t>(ids), static_cast<int32_t>(K), ptr(probs), ptr(stats), ptr(gl),
+                                       stride, out[0].data_ptr(), stream_of(z)), "ltc_distill_loss backward");
       }
     }
     return once(std::move(out), std::move(inputs));
@@ -408,7 +451,7 @@ struct ScoresFunction : torch::autograd::Function<ScoresFunction> {
     auto [lp, ent, ids, best, stats] = scores_forward(z, tokens, r, k, true);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({z, tokens, stats});
-    keep_rows(ctx, r);
+    keep_rows(ctx, z, r);
     if (!k) return {lp, ent};
     ctx->mark_non_differentiable({ids, best});
     return {lp, ent, ids, best};
@@ -418,16 +461,17 @@ struct ScoresFunction : torch::autograd::Function<ScoresFunction> {
     {
       const at::NoGradGuard no_grad;
       const auto v = ctx->get_saved_variables();
-      const Tensor& z = v[0];
-      inputs = {z};
-      const Rows r = kept_rows(ctx);
+      inputs = {v[0]};
+      const auto [z, r] = kept_rows(ctx, v[0]);
+      const Tensor tokens = restored(v[1], at::kLong, r.n[0], z.device());
+      const Tensor stats = restored(v[2], at::kFloat, r.n[0] * 4, z.device());
       out[0] = fresh(z);
       if (r.n[0]) {
         const c10::cuda::CUDAGuard guard(z.device());
         const auto [glp, slp] = row_grad(g[0], r.n[0]);
         const auto [gent, sent] = row_grad(g[1], r.n[0]);
         const LtcLogits l = logits_of(z, r);
-        check(lib.ltc_token_logprobs_backward(&l, ptr<int64_t>(v[1]), ptr(v[2]), ptr(glp), slp, ptr(gent), sent,
+        check(lib.ltc_token_logprobs_backward(&l, ptr<int64_t>(tokens), ptr(stats), ptr(glp), slp, ptr(gent), sent,
                                               out[0].data_ptr(), stream_of(z)), "ltc_token_logprobs backward");
       }
     }
