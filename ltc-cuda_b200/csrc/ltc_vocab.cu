@@ -249,7 +249,7 @@ struct TopShared {
   float warp_v[NT / 32];
   int warp_i[NT / 32];
   int count;
-  float pv, thr;
+  float pv, thr, thr_all;
   int pi;
 };
 struct NoShared {};
@@ -448,14 +448,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
   }
 
   if constexpr (TOPK) {
-    float thr = top.thr;
+    float thr = top.thr;  // every warp branches on it below, so nothing writes it any more
     if (thr == neg_inf() && t.m != neg_inf()) {
       // short or masked rows leave warps without values: the k-th largest of all thread maxima instead
       int above = 0;
       for (int d = 0; d < NT; ++d) above += better(top.thread_v[d], d, best, tid) ? 1 : 0;
-      if (above == g.k - 1) top.thr = best;
+      if (above == g.k - 1) top.thr_all = best;
       __syncthreads();
-      thr = top.thr;
+      thr = top.thr_all;
     }
     auto reaches = [&](float v) { return v >= thr && v > neg_inf(); };
     auto keep = [&](float v, int i) {
