@@ -17,7 +17,9 @@
 // the next tile's loads are in flight while this one is combined and written.  Where there
 // are too few items to fill the GPU, a cluster of up to 16 blocks takes one item, block r the
 // tiles r, r + cl, ...: every round the blocks' folds go to every block's shared memory as
-// messages that complete bytes on the receiver's mbarrier (bounded waits).  All orders are
+// messages that complete bytes on the receiver's mbarrier (bounded waits; a block whose wait
+// expired sends and arms no more, so that the others' waits expire as well, and no block leaves
+// before all are done).  All orders are
 // fixed: results do not depend on scheduling.
 //
 // Backward.  The forward leaves the state before every 32nd token (fp32); the backward
@@ -327,13 +329,19 @@ __device__ __forceinline__ void exchange_begin(Exchange<NW, NF, true>& sh, int c
   cg::this_cluster().sync();
 }
 
+// behind the last round: no block leaves while another may still address its shared memory, which
+// the message counts alone ensure only as long as no wait expires
+__device__ __forceinline__ void exchange_end(int cl) {
+  if (cl > 1) cg::this_cluster().sync();
+}
+
 // The warps' folds are in shared memory: makes them visible to the block and sends the block's
 // fold (in time order) to all blocks of the cluster, each warp to its share of them.  The
 // messages complete bytes on the receiver's barrier, so that no block waits for its own.
 template <bool PACKED, bool REVERSE, int NW, int NF, bool MANY>
 __device__ __forceinline__ void exchange_send(Exchange<NW, NF, MANY>& sh, int buf, int cl, int rank) {
   __syncthreads();
-  if (!MANY || cl == 1) return;
+  if (!MANY || cl == 1 || *static_cast<volatile int*>(&sh.aborted)) return;
   const int ch = threadIdx.x & 31;  // a narrow item's upper half sends what nobody reads
   float A = 1.f, B = 0.f;
   int F = 0;
@@ -363,7 +371,7 @@ __device__ __forceinline__ void exchange_wait(Exchange<NW, NF, MANY>& sh, int bu
   if (!MANY || cl == 1) return;
   const unsigned bar = smem_addr(&sh.bar[buf]);
   mbar_wait(bar, phase, &sh.aborted, &g_scan_wait_timeouts);
-  if (threadIdx.x == 0) mbar_arm(bar, message_bytes(cl));
+  if (threadIdx.x == 0 && !*static_cast<volatile int*>(&sh.aborted)) mbar_arm(bar, message_bytes(cl));
 }
 
 // (A, B) of this thread's channels
@@ -670,6 +678,7 @@ __global__ void __launch_bounds__(S::THREADS, (fwd_blocks<P, T, S, MANY>())) sca
     m = next;
   }
 
+  if constexpr (MANY) exchange_end(cl);
   if (!chok || it.rank != 0) return;
   if (!PACKED) {
     if (ty == 0) store(g.hT + b * g.H + ch, carry);
@@ -940,6 +949,7 @@ __global__ void __launch_bounds__(S::THREADS, (bwd_blocks<P, T, S, MANY>())) sca
     }
   }
 
+  if constexpr (MANY) exchange_end(cl);
   if (P) {  // decay gradient of this block or warp: fixed order over the time groups
     if (S::GPW > 1) acc = vadd(acc, vxor(acc, LX % 32));
     if (NW > 1) {
