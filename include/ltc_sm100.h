@@ -205,7 +205,7 @@ enum { LTC_DTYPE_F32 = 0, LTC_DTYPE_BF16 = 1, LTC_DTYPE_F16 = 2 };
  *   gated    L_t = -scale softplus(decay) sigmoid(rate_t),  a_t = exp(L_t),
  *            h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(gate_t) x_t
  * Padded batches: inputs (B,T,H), states (B,H), num_seqs = 0, seq_starts NULL.
- * Packed sequences: B = 1, T = all tokens, num_seqs = S >= 1, states (S,H), and seq_starts
+ * Packed sequences: B = 1, T = all tokens, num_seqs = S in 1..2^30, states (S,H), and seq_starts
  * (S+1) non-decreasing token offsets ON THE DEVICE: sequence n holds tokens seq_starts[n] ..
  * seq_starts[n+1]-1 (none: its first state is its final state).  Tokens outside every
  * sequence give h = 0 and zero gradients, whatever they hold.  Offsets out of order give

@@ -899,6 +899,7 @@ int scan_begin(const LtcScanDims* d, const char* who, ScanCall* c) {
   if (d->dtype < 0 || d->dtype > LTC_DTYPE_F16) return fail("%s: unknown dtype %d", who, d->dtype);
   if (d->H > kScanMaxH) return fail("%s: at most %d channels", who, kScanMaxH);
   if (d->num_seqs < 0 || (d->num_seqs > 0 && d->B != 1)) return fail("%s: packed sequences need B = 1", who);
+  if (d->num_seqs > kScanMaxS) return fail("%s: at most %d packed sequences", who, kScanMaxS);
   int err = 0;
   c->di = device_info(&err);
   if (err) return 1;

@@ -211,6 +211,7 @@ cudaError_t launch_preamble_bwd(const PreambleArgs& a, int num_sms, cudaStream_t
 constexpr int kScanShort = 16;       // rows up to this length are one tile of one warp
 constexpr int kScanBound = 32;       // the forward saves the state before every so many tokens
 constexpr int kScanMaxT = 0x7fff0000;  // time steps: a round past the end still fits 31 bits
+constexpr int kScanMaxS = 1 << 30;   // packed sequences: the sum of two of their indices fits 31 bits
 constexpr int kScanMaxH = 1 << 28;   // channels, and time strides: byte offsets of a row fit 32 bits
 constexpr int kScanMaxCluster = 16;  // blocks that share one item (sequence x 32 channels)
 struct ScanArgs {

@@ -705,6 +705,7 @@ def ltc_preamble(x, ln_w, ln_b, in_w, in_b, eps: float):
 SCAN_MAX_H = 1 << 28
 SCAN_MAX_T = 0x7fff0000
 SCAN_MAX_B = 0x7fffffff
+SCAN_MAX_S = 1 << 30  # packed sequences: the search among their offsets adds two of their indices
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -765,7 +766,9 @@ def _scan_operands(names, tensors, h0, seq_starts):
             raise ValueError(f"seq_starts is on {seq_starts.device}, expected {first.device}")
         T, H = first.shape
         B, S = 1, seq_starts.numel() - 1
-    _check_batch(S or B)
+    if S > SCAN_MAX_S:
+        raise ValueError(f"more than 2^30 packed sequences (got {S})")
+    _check_batch(B)
     if T > SCAN_MAX_T or H > SCAN_MAX_H or any(t.stride(-2) > SCAN_MAX_H for t in tensors):
         raise ValueError("more than 2^31 - 2^16 time steps, 2^28 channels, or a time stride past 2^28 elements")
     if h0 is not None:

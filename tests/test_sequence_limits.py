@@ -1,0 +1,33 @@
+"""CPU: the sequence operators' limits, at the value that is still taken and the first that is not."""
+import ctypes
+
+import pytest
+import torch
+
+import ltc_cuda
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def test_packed_sequences_past_2_30_are_refused(monkeypatch):
+    """The search among the offsets adds two sequence indices: past 2^30 the sum wraps to an offset
+    in front of the array."""
+    args = t(4, 3), t(4, 3)
+    for n in ((1 << 30) + 1, (1 << 31) - 1):
+        starts = t(1, dtype=torch.int32).expand(n + 1)
+        with pytest.raises(ValueError, match="sequences"):
+            ltc_cuda.ltc_linear_scan(*args, seq_starts=starts)
+    with pytest.raises(ValueError, match="the sm_100a kernels need CUDA"):  # taken, up to the device
+        ltc_cuda.ltc_linear_scan(*args, seq_starts=t(1, dtype=torch.int32).expand((1 << 30) + 1))
+    lib = ltc_cuda._lib
+    if lib is None:
+        pytest.skip("library not built")
+    dims = ltc_cuda.LtcScanDims(1, 4, 3, 0, (1 << 30) + 1)
+    assert lib.ltc_scan_plan(ctypes.byref(dims), ctypes.byref(ltc_cuda.LtcScanPlan())) != 0
+    assert b"packed sequences" in lib.ltc_last_error()
+    # one fewer gets as far as the device
+    dims.num_seqs -= 1
+    lib.ltc_scan_plan(ctypes.byref(dims), ctypes.byref(ltc_cuda.LtcScanPlan()))
+    assert b"packed sequences" not in lib.ltc_last_error()
