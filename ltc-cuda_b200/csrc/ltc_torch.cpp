@@ -306,7 +306,7 @@ py::object gated_step(py::handle x_, py::handle rate_, py::handle gate_, py::han
   Tensor out;
   if (given) {
     out = THPVariable_Unpack(out_.ptr());
-    if (!is_floats(out, x, x.sizes())) return py::none();
+    if (!is_floats(out, x, x.sizes()) || wants_grad({out})) return py::none();
     const intptr_t apart = static_cast<char*>(out.data_ptr()) - static_cast<char*>(state.data_ptr());
     if (apart != 0 && std::abs(apart) < 4 * state.numel()) return py::none();
   }
@@ -314,7 +314,8 @@ py::object gated_step(py::handle x_, py::handle rate_, py::handle gate_, py::han
   {
     const py::gil_scoped_release release;
     h = fresh(x);
-    if (!given) out = floats(x, x.sizes());
+    if (given) out.unsafeGetTensorImpl()->bump_version();  // an earlier graph that keeps it has to notice
+    else out = floats(x, x.sizes());
     if (h.numel()) {
       const c10::cuda::CUDAGuard guard(x.device());
       const LtcScanDims d{static_cast<int32_t>(B), 1, static_cast<int32_t>(H), dtype_of(x), 0};
