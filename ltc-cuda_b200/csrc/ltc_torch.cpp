@@ -99,6 +99,13 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     if (t.defined() && t.requires_grad()) return true;
   return false;
 }
+// Forward-mode derivatives do not exist here, and a dropped tangent would read as a zero one.
+void refuse_tangents(std::initializer_list<Tensor> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor& t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(),
+                                "ltc_cuda: the sequence operators have no forward-mode derivative");
+}
 // Saved tensors come back as a saved-tensor hook left them (offloaded, repacked): the values are the
 // forward's, the layout need not be.  `t` as a contiguous array of the forward's type and length.
 Tensor restored(const Tensor& t, at::ScalarType type, int64_t n, const at::Device& on) {
@@ -265,6 +272,7 @@ std::pair<Tensor, Tensor> scan(const OptTensor& decay_, const OptTensor& h0_, co
   const Tensor x2 = or_none(third);
   const Scan s{{static_cast<int32_t>(n[0]), static_cast<int32_t>(n[1]), static_cast<int32_t>(n[2]), dtype_of(in[0]),
                 static_cast<int32_t>(n[3])}, scale, decay.defined()};
+  refuse_tangents({in[0], in[1], x2, decay, h0});
   if (wants_grad({in[0], in[1], x2, decay, h0})) {
     auto r = ScanFunction::apply(s, decay_, h0_, starts_, in[0], in[1], third);
     return {r[0], r[1]};
@@ -302,6 +310,7 @@ py::object gated_step(py::handle x_, py::handle rate_, py::handle gate_, py::han
         (t->stride(1) != 1 && H != 1))
       return py::none();
   if (!is_floats(decay, x, {H}) || !is_floats(state, x, x.sizes())) return py::none();
+  refuse_tangents({x, rate, gate, decay, state});
   if (wants_grad({x, rate, gate, decay, state})) return py::none();
   Tensor out;
   if (given) {
@@ -421,6 +430,7 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
 Tensor distill(const Tensor& z, const Tensor& ids, const Tensor& teacher, const std::array<int64_t, 4>& rows,
                double temperature) {
   const Rows r{rows, temperature};
+  refuse_tangents({z});
   if (wants_grad({z})) return DistillFunction::apply(z, ids, teacher, r);
   return distill_forward(z, ids, teacher, r, false)[0];
 }
@@ -484,6 +494,7 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> scores(const Tensor& z, const T
                                                         const std::array<int64_t, 4>& rows, double temperature,
                                                         int64_t k) {
   const Rows r{rows, temperature};
+  refuse_tangents({z});
   if (wants_grad({z})) {
     auto v = ScoresFunction::apply(z, tokens, r, k);
     if (!k) return {v[0], v[1], std::nullopt, std::nullopt};

@@ -60,3 +60,28 @@ def test_step_on_inference_tensors():
     with pytest.raises(RuntimeError, match="InferenceMode"):
         ltc_cuda.ltc_gated_scan_step(x, x, x, decay, state, out_state=state)
     assert torch.equal(state, want)
+
+
+def test_forward_mode_is_refused():
+    """No tangent comes out, so none may go in, whether or not gradients are recorded."""
+    from torch.autograd import forward_ad
+    x, decay, state, z = normal(2, 9, 8), normal(8, seed=1), normal(2, 8, seed=2), normal(4, 33, seed=3)
+    ids = torch.zeros(4, 2, dtype=torch.int64, device="cuda")
+    calls = [
+        lambda d: ltc_cuda.ltc_linear_scan(x, d(x)), lambda d: ltc_cuda.ltc_linear_scan(x, x, d(state)),
+        lambda d: ltc_cuda.ltc_gated_scan(x, x, x, d(decay)), lambda d: ltc_cuda.ltc_gated_scan(x, d(x), x, decay),
+        lambda d: ltc_cuda.ltc_gated_scan_step(x[:, 0], d(x[:, 0]), x[:, 0], decay, state),
+        lambda d: ltc_cuda.ltc_gated_scan_step(x[:, 0], x[:, 0], x[:, 0], decay, d(state)),
+        lambda d: ltc_cuda.ltc_distill_loss(d(z), ids, z[:, :2]),
+        lambda d: ltc_cuda.ltc_token_logprobs(d(z), ids[:, 0], top_k=2),
+    ]
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in calls:
+            call(lambda t: t)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
+        with forward_ad._set_fwd_grad_enabled(False):  # nothing is recorded, as in PyTorch's operations
+            calls[0](dual)
