@@ -217,7 +217,8 @@ typedef struct {
   int32_t num_seqs; /* 0: padded batch */
 } LtcScanDims;
 
-/* One (B,T,H) input: element strides of batch and time, channels contiguous. */
+/* One (B,T,H) input: element strides of batch and time (at most 2^28, not used where T is 1),
+ * channels contiguous. */
 typedef struct {
   const void* data;
   int64_t stride_b, stride_t;

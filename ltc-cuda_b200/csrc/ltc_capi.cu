@@ -914,8 +914,9 @@ int scan_begin(const LtcScanDims* d, const char* who, ScanCall* c) {
 size_t scan_workspace(const ScanCall& c, bool bwd) { return bwd ? c.part_floats * sizeof(float) : 0; }
 
 int scan_strides(const LtcScanDims* d, const char* who, const LtcScanInput* in, int i, ScanArgs* a) {
-  const int64_t bytes = in->stride_t * (d->dtype == LTC_DTYPE_F32 ? 4 : 2);
-  if (in->stride_t < -(1 << 28) || in->stride_t > (1 << 28)) return fail("%s: a time stride is past 2^28", who);
+  const int64_t stride_t = d->T == 1 ? 0 : in->stride_t;  // a single time step has no use for it
+  const int64_t bytes = stride_t * (d->dtype == LTC_DTYPE_F32 ? 4 : 2);
+  if (stride_t < -(1 << 28) || stride_t > (1 << 28)) return fail("%s: a time stride is past 2^28", who);
   a->sb[i] = in->stride_b;
   a->st[i] = (int)bytes;
   return 0;
@@ -1092,7 +1093,6 @@ int ltc_gated_scan_step(const LtcScanDims* dims, const LtcScanInput* x, const Lt
   ScanArgs a{};
   if (scan_args(&d, c, who, in, 3, state, nullptr, false, nullptr, 0, &a)) return 1;
   if (!h || !state_out || !decay) return fail("%s: NULL pointer", who);
-  for (int i = 0; i < 3; ++i) a.st[i] = 0;
   a.decay = decay; a.scale = scale;
   a.h = h; a.hT = state_out;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

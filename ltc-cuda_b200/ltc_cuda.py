@@ -769,7 +769,7 @@ def _scan_operands(names, tensors, h0, seq_starts):
     if S > SCAN_MAX_S:
         raise ValueError(f"more than 2^30 packed sequences (got {S})")
     _check_batch(B)
-    if T > SCAN_MAX_T or H > SCAN_MAX_H or any(t.stride(-2) > SCAN_MAX_H for t in tensors):
+    if T > SCAN_MAX_T or H > SCAN_MAX_H or (T > 1 and any(t.stride(-2) > SCAN_MAX_H for t in tensors)):
         raise ValueError("more than 2^31 - 2^16 time steps, 2^28 channels, or a time stride past 2^28 elements")
     if h0 is not None:
         h0 = _as_f32(h0, first.device, "h0")

@@ -51,3 +51,27 @@ def test_clusters_close_together(op, T, H, cluster):
             assert_within(h, *ref["h"], "h")
         assert all(torch.isfinite(t.grad).all() for t in leaves.values())
     assert ltc_cuda.wait_timeouts() == 0
+
+
+def test_wide_rows_of_one_time_step():
+    """One position of a projection whose rows are more than 2^28 elements apart: a step, and a scan of T = 1."""
+    H, apart = 8, (1 << 28) + 16
+    store = torch.zeros(apart + 3 * H, device="cuda", dtype=torch.float16)
+    g = torch.Generator().manual_seed(0)
+    rows = torch.randn(2, 3 * H, generator=g).half().cuda()
+    store[:3 * H], store[apart:] = rows[0], rows[1]
+    wide = store.as_strided((2, 3 * H), (apart, 1))
+    decay, state = torch.randn(H, generator=g).cuda() - 3, torch.randn(2, H, generator=g).cuda()
+    want = ltc_cuda.ltc_gated_scan_step(*rows.split(H, dim=1), decay, state)
+    got = ltc_cuda.ltc_gated_scan_step(*wide.split(H, dim=1), decay, state)
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
+    leaf = rows[:, None].clone().requires_grad_(True)  # T = 1, with a time stride that means nothing
+    far = [t.as_strided((2, 1, H), (apart, apart, 1), t.storage_offset()) for t in wide.split(H, dim=1)]
+    for t in far:
+        t.requires_grad_(True)
+    h, last = ltc_cuda.ltc_gated_scan(*far, decay, state)
+    hw, lw = ltc_cuda.ltc_gated_scan(*leaf.split(H, dim=2), decay, state)
+    assert torch.equal(h, hw) and torch.equal(last, lw) and torch.equal(last, want[1])
+    grads = torch.autograd.grad([h, last], far, [torch.ones_like(h), torch.ones_like(last)])
+    (gw,) = torch.autograd.grad([hw, lw], [leaf], [torch.ones_like(h), torch.ones_like(last)])
+    assert torch.equal(torch.cat(grads, 2), gw)

@@ -31,3 +31,16 @@ def test_packed_sequences_past_2_30_are_refused(monkeypatch):
     dims.num_seqs -= 1
     lib.ltc_scan_plan(ctypes.byref(dims), ctypes.byref(ltc_cuda.LtcScanPlan()))
     assert b"packed sequences" not in lib.ltc_last_error()
+
+
+def test_time_stride_of_a_single_step_is_not_looked_at(monkeypatch):
+    """Past 2^28 elements a time stride is refused, but one step has no use for any."""
+    monkeypatch.setattr(ltc_cuda, "_on_cuda", lambda *_: None)
+    one = t(1).as_strided((1, 1, 1), (1, (1 << 28) + 1, 1))
+    (a, _), _, _, dims = ltc_cuda._scan_operands(("a", "b"), (one, one), None, None)
+    assert a.stride(1) > 1 << 28 and dims == (1, 1, 1, 0)
+    two = torch.empty(1).as_strided((1, 1, 1), (1, 1, 1)).expand(1, 2, 1)
+    ltc_cuda._scan_operands(("a", "b"), (two, two), None, None)
+    wide = torch.empty(((1 << 28) + 2,), dtype=torch.float16).as_strided((1, 2, 1), (1, (1 << 28) + 1, 1))
+    with pytest.raises(ValueError, match="time stride"):
+        ltc_cuda._scan_operands(("a", "b"), (wide, wide), None, None)
