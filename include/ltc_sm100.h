@@ -208,8 +208,9 @@ enum { LTC_DTYPE_F32 = 0, LTC_DTYPE_BF16 = 1, LTC_DTYPE_F16 = 2 };
  * Packed sequences: B = 1, T = all tokens, num_seqs = S in 1..2^30, states (S,H), and seq_starts
  * (S+1) non-decreasing token offsets ON THE DEVICE: sequence n holds tokens seq_starts[n] ..
  * seq_starts[n+1]-1 (none: its first state is its final state).  Tokens outside every
- * sequence give h = 0 and zero gradients, whatever they hold.  Offsets out of order give
- * wrong numbers but no access out of bounds.  Runs of tokens are folded by their products of
+ * sequence give h = 0 and zero gradients, whatever they hold.  Offsets below 0 count as 0,
+ * offsets past T as T.  Offsets out of order make every final state and every gradient of a
+ * first state NaN, the rest wrong, and cause no access out of bounds.  Runs of tokens are folded by their products of
  * a: one over 128 tokens past fp32's range gives infinities or NaN (|a| <= 1 is safe). */
 typedef struct {
   int32_t B, T, H;

@@ -208,6 +208,11 @@ __device__ __forceinline__ int seq_of(const int* starts, int S, int t) {
   return lo;
 }
 
+// offset n as far as there are tokens
+__device__ __forceinline__ int offset_of(const int* starts, int n, int T) {
+  return min(max(__ldg(starts + n), 0), T);
+}
+
 struct Marks {         // of a thread's R tokens, one bit each
   unsigned first = 0;  // starts its sequence
   unsigned last = 0;   // ends it
@@ -225,15 +230,15 @@ __device__ __forceinline__ int seq_at(unsigned bits, int n, int j, const int* st
 // one sequence.
 struct Walk {
   const int* starts;
-  int S, stride, pick, begin, end;
+  int S, T, stride, pick, begin, end;
   int n = 0, s0 = 0, s1 = 0;  // sequence of the last tile, its tokens [s0, s1)
 
-  __device__ __forceinline__ Walk(const int* starts_, int S_, int T) : starts(starts_), S(S_) {
+  __device__ __forceinline__ Walk(const int* starts_, int S_, int T_) : starts(starts_), S(S_), T(T_) {
     stride = (S + 31) / 32;
     const int at = (int)(threadIdx.x & 31) * stride;
     pick = at < S ? __ldg(starts + at) : 0x7fffffff;
-    begin = __ldg(starts);
-    end = min(__ldg(starts + S), T);
+    begin = offset_of(starts, 0, T);
+    end = offset_of(starts, S, T);
   }
   // all lanes of a warp call it with the same tile
   __device__ __forceinline__ void find(int t) {
@@ -246,8 +251,8 @@ struct Walk {
     }
     n = min(block + max(count - 1, 0), S - 1);
     LTC_CHECK(n >= 0 && n < S, 901);
-    s0 = __ldg(starts + n);
-    s1 = __ldg(starts + n + 1);
+    s0 = offset_of(starts, n, T);
+    s1 = offset_of(starts, n + 1, T);
   }
   template <int R, int TT>
   __device__ __forceinline__ Marks marks(int tile_t0, int t0) {
@@ -272,7 +277,7 @@ struct Walk {
       if (b >= t0 + R || k + 1 >= S) break;
       ++k;
       a = b;
-      b = __ldg(starts + k + 1);
+      b = offset_of(starts, k + 1, T);
     }
     return m;
   }
@@ -284,6 +289,23 @@ struct NoWalk {
 };
 template <bool PACKED> struct WalkOf { using type = NoWalk; };
 template <> struct WalkOf<true> { using type = Walk; };
+
+// A block's last act on the states of its channels, behind every other write to them: a sequence
+// without a token passes `from` on (its first state; backward: the gradient of its final one).
+// Offsets out of order leave sequences unvisited: then all rows become NaN, not what was in memory.
+// All threads of the block call it.
+template <typename V, int TY>
+__device__ __forceinline__ void finish_sequences(const ScanArgs& g, float* to, const float* from, int ch, bool chok,
+                                                 int ty) {
+  bool disorder = false;
+  for (int n = ty; n < g.S; n += TY) {
+    disorder |= __ldg(g.starts + n) > __ldg(g.starts + n + 1);
+    if (chok && offset_of(g.starts, n, g.T) >= offset_of(g.starts, n + 1, g.T))
+      store(to + (long long)n * g.H + ch, from ? load_f32<V>(from + (long long)n * g.H + ch) : V{});
+  }
+  if (!__syncthreads_or(disorder) || !chok) return;
+  for (int n = ty; n < g.S; n += TY) store(to + (long long)n * g.H + ch, all_of<V>(__int_as_float(0x7fffffff)));
+}
 
 // ---- shapes ----------------------------------------------------------------------
 template <int VEC_, int R_, int TY_, int BB_, int ITEM_ = kItem>
@@ -679,14 +701,9 @@ __global__ void __launch_bounds__(S::THREADS, (fwd_blocks<P, T, S, MANY>())) sca
   }
 
   if constexpr (MANY) exchange_end(cl);
-  if (!chok || it.rank != 0) return;
-  if (!PACKED) {
-    if (ty == 0) store(g.hT + b * g.H + ch, carry);
-    return;
-  }
-  for (int n = ty; n < g.S; n += S::TY)  // sequences without a token pass their first state on
-    if (__ldg(g.starts + n) >= __ldg(g.starts + n + 1))
-      store(g.hT + (long long)n * g.H + ch, g.h0 ? load_f32<V>(g.h0 + (long long)n * g.H + ch) : V{});
+  if (it.rank != 0) return;
+  if constexpr (PACKED) finish_sequences<V, S::TY>(g, g.hT, g.h0, ch, chok, ty);
+  else if (chok && ty == 0) store(g.hT + b * g.H + ch, carry);
 }
 
 // blocks that an SM's registers have to hold; more spill (bf16 gated: 5 against 4 blocks 184 and 205 us at
@@ -962,14 +979,9 @@ __global__ void __launch_bounds__(S::THREADS, (bwd_blocks<P, T, S, MANY>())) sca
     }
     if (chok && ty == 0) store(g.part + (b * cl + it.rank) * g.H + ch, acc);
   }
-  if (!chok || it.rank != 0 || !g.dh0) return;
-  if (!PACKED) {
-    if (ty == 0) store(g.dh0 + b * g.H + ch, carry);
-    return;
-  }
-  for (int n = ty; n < g.S; n += S::TY)
-    if (__ldg(g.starts + n) >= __ldg(g.starts + n + 1))
-      store(g.dh0 + (long long)n * g.H + ch, g.dhT ? load_f32<V>(g.dhT + (long long)n * g.H + ch) : V{});
+  if (it.rank != 0 || !g.dh0) return;
+  if constexpr (PACKED) finish_sequences<V, S::TY>(g, g.dh0, g.dhT, ch, chok, ty);
+  else if (chok && ty == 0) store(g.dh0 + b * g.H + ch, carry);
 }
 
 // d loss / d decay = -scale sigmoid(decay) * sum of the items' partial sums, in fixed order

@@ -777,6 +777,8 @@ def _scan_operands(names, tensors, h0, seq_starts):
             raise ValueError(f"h0 has shape {tuple(h0.shape)}, expected {(S or B, H)}")
     _on_cuda(first, names[0])
     if seq_starts is not None:
+        if seq_starts.dtype == torch.int64:
+            seq_starts = seq_starts.clamp(0, T)  # an offset past 31 bits must not wrap
         seq_starts = seq_starts.to(torch.int32).contiguous()
     return [_rows(t) for t in tensors], h0, seq_starts, (B, T, H, S)
 
@@ -802,7 +804,8 @@ def ltc_linear_scan(a, b, h0=None, seq_starts=None) -> Tuple[torch.Tensor, torch
     same, any batch and time strides.  ``h0`` (fp32 ``(B, H)`` or ``(S, H)``) defaults to
     zeros.  ``h`` has the type of the inputs, ``h_final`` is fp32, and so is the state in
     between.  Tokens that belong to no sequence give 0 and get no gradient; a sequence
-    without tokens returns its ``h0``.  Runs of tokens are folded by their products of ``a``:
+    without tokens returns its ``h0``.  Offsets end at the last token; offsets out of order
+    make every ``h_final`` and every gradient of ``h0`` NaN.  Runs of tokens are folded by their products of ``a``:
     a product over 128 tokens past fp32's range gives infinities or NaN even where the state
     is 0 (``|a| <= 1`` is always safe).  Differentiable once in ``a``, ``b`` and ``h0``."""
     tensors, h0, seq_starts, dims = _scan_operands(("a", "b"), (a, b), h0, seq_starts)

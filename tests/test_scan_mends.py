@@ -75,3 +75,52 @@ def test_wide_rows_of_one_time_step():
     grads = torch.autograd.grad([h, last], far, [torch.ones_like(h), torch.ones_like(last)])
     (gw,) = torch.autograd.grad([hw, lw], [leaf], [torch.ones_like(h), torch.ones_like(last)])
     assert torch.equal(torch.cat(grads, 2), gw)
+
+
+def gradients(op, args, h0, dh, dlast, starts):
+    leaves = {n: t.clone().requires_grad_(True) for n, t in args.items()}
+    first = h0.clone().requires_grad_(True)
+    h, last = run(op, leaves, first, starts)
+    grads = torch.autograd.grad([h, last], [*leaves.values(), first], [dh, dlast])
+    return {"h": h, "state": last, **{"d" + n: g for n, g in zip([*leaves, "h0"], grads)}}
+
+
+def dirty_memory(*like):
+    """What the allocator hands out next has been written before."""
+    held = [torch.full_like(t, 1e30) for t in like for _ in range(8)]
+    torch.cuda.synchronize()
+    del held
+
+
+@pytest.mark.parametrize("op", ["linear", "gated"])
+@pytest.mark.parametrize("H", [12, 5])
+@pytest.mark.parametrize("starts,N,wide", [
+    ([0, 40, 90], 70, False), ([-5, 30, 200, 300], 130, False), ([0, 700, 5000, 6000], 1500, False),
+    ([0, 64, 128, 129], 128, False), ([0, 30, (1 << 32) + 7, 1 << 40], 90, True)])
+def test_offsets_end_at_the_tokens(op, starts, N, wide, H):
+    """A sequence that reaches past the tokens ends with them, one behind them has none; int64
+    offsets do not wrap.  Both kinds of state rows are written."""
+    S = len(starts) - 1
+    args = operands(op, (N,), H, N + H)
+    g = torch.Generator().manual_seed(N)
+    h0, dh, dlast = (torch.randn(*s, generator=g).cuda() for s in ((S, H), (N, H), (S, H)))
+    t = torch.tensor(starts, device="cuda", dtype=torch.int64 if wide else torch.int32)
+    dirty_memory(h0, dh)
+    got = gradients(op, args, h0, dh, dlast, t)
+    ref = scan_reference(op, args, h0, dh, dlast, [min(max(s, 0), N) for s in starts])
+    for n, v in got.items():
+        assert_within(v, *ref[n], n)
+
+
+@pytest.mark.parametrize("op", ["linear", "gated"])
+@pytest.mark.parametrize("starts,N", [([0, 100, 50, 60], 200), ([90, 3, 500, -7, 20], 400), ([10, 5], 40),
+                                      ([0, 1500, 300, 2000], 2000)])
+def test_offsets_out_of_order_give_nan_states(op, starts, N):
+    """Never what was in memory before: states and their gradients are NaN, all of them."""
+    S, H = len(starts) - 1, 20
+    args = operands(op, (N,), H, N)
+    h0 = torch.zeros(S, H, device="cuda")
+    t = torch.tensor(starts, device="cuda", dtype=torch.int32)
+    dirty_memory(h0)
+    got = gradients(op, args, h0, torch.ones(N, H, device="cuda"), torch.ones(S, H, device="cuda"), t)
+    assert got["state"].isnan().all() and got["dh0"].isnan().all()
