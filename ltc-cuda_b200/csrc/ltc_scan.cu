@@ -274,10 +274,14 @@ struct Walk {
           m.last |= 1u << (b - 1 - t0);
         }
       }
-      if (b >= t0 + R || k + 1 >= S) break;
+      if (b >= t0 + R || b >= end || k + 1 >= S) break;
       ++k;
       a = b;
       b = offset_of(starts, k + 1, T);
+      if (b <= a) {  // no token: on to the last sequence that starts here, however many there are
+        k = max(k, seq_of(starts, S, a));
+        b = offset_of(starts, k + 1, T);
+      }
     }
     return m;
   }

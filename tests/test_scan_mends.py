@@ -124,3 +124,44 @@ def test_offsets_out_of_order_give_nan_states(op, starts, N):
     dirty_memory(h0)
     got = gradients(op, args, h0, torch.ones(N, H, device="cuda"), torch.ones(S, H, device="cuda"), t)
     assert got["state"].isnan().all() and got["dh0"].isnan().all()
+
+
+def many_sequences(kind, N):
+    g = torch.Generator().manual_seed(7)
+    if kind == "short":  # about 1600 sequences of 0 to 3 tokens: lanes search more than 32 offsets each
+        lens = torch.randint(0, 4, (1600,), generator=g)
+        starts = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)])
+        return [int(s) for s in starts if s <= N]
+    if kind == "runs of empty ones":  # inside tiles, between their threads, at both ends
+        at = torch.tensor([0, 5, 37, 63, 64, 130, 131, N - 1, N]).repeat_interleave(400)
+        return at.tolist()
+    return [0, 3] + [70] * 20000 + [100, 100, N]  # one offset, inside a tile
+
+
+@pytest.mark.parametrize("op", ["linear", "gated"])
+@pytest.mark.parametrize("N,H", [(700, 5), (2300, 12)])
+@pytest.mark.parametrize("kind", ["short", "runs of empty ones", "one offset"])
+def test_more_than_1024_sequences(op, N, H, kind):
+    starts = many_sequences(kind, N)
+    S = len(starts) - 1
+    args = operands(op, (N,), H, S)
+    g = torch.Generator().manual_seed(S)
+    h0, dh, dlast = (torch.randn(*s, generator=g).cuda() for s in ((S, H), (N, H), (S, H)))
+    got = gradients(op, args, h0, dh, dlast, torch.tensor(starts, device="cuda", dtype=torch.int32))
+    ref = scan_reference(op, args, h0, dh, dlast, starts)
+    for n, v in got.items():
+        assert_within(v, *ref[n], n)
+
+
+def test_many_empty_sequences_are_stepped_over():
+    """A million empty sequences at one offset inside a tile, while the cluster's other blocks wait
+    for it: no bounded wait expires, and the tokens are those of the two sequences around them."""
+    N, H, S = 2000, 16, 1000002
+    assert cluster_of(1, N, H, S) > 1
+    args = operands("gated", (N,), H, 3)
+    starts = torch.full((S + 1,), 1030, dtype=torch.int32, device="cuda")
+    starts[0], starts[-1] = 0, N
+    h, last = run("gated", args, None, starts)
+    want, wl = run("gated", args, None, torch.tensor([0, 1030, N], dtype=torch.int32, device="cuda"))
+    assert torch.equal(h, want) and torch.equal(last[[0, -1]], wl) and bool((last[1:-1] == 0).all())
+    assert ltc_cuda.wait_timeouts() == 0
