@@ -42,7 +42,10 @@ constexpr int kUnroll = 4;     // 16-byte loads in flight per thread
 constexpr int kCap = 1024;     // candidates for the k best
 constexpr int kSlots = 16;     // noted maxima per thread; longer rows note several windows as one
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kFar = -1e30f; // stands for -inf where a zero weight multiplies it
+// Stands for everything below it where 2^y multiplies it: 2^y is 0 from y = -127 on (ex2 flushes), and
+// small enough that a factor of up to 3e35 (a large loss scale over a small temperature) leaves the product
+// finite.
+constexpr float kFar = -1024.f;
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
   float y;

@@ -27,3 +27,34 @@ def test_alternatives_where_warps_hold_no_values(rows, V, left, dtype):
         want = torch.where(order.values[:, :k] > -INF, order.indices[:, :k], -1)
         for _ in range(5):
             assert torch.equal(ltc_cuda.ltc_token_logprobs(z, tokens, top_k=k).top_ids, want)
+
+
+@pytest.mark.parametrize("V", [33, 5000])
+@pytest.mark.parametrize("exponent", [0, -30, -60])
+def test_entropy_gradient_of_masked_rows_under_large_factors(V, exponent):
+    """A loss scale of 2^40 over temperatures down to 2^-60: powers of two, so every value is that
+    of the plain call times the factor, bit by bit, and masked entries get 0."""
+    g = torch.Generator().manual_seed(V)
+    z = torch.randn(4, V, generator=g).cuda() * 3
+    z[0, ::3] = -INF
+    z[1, 1:] = -INF
+    z[2, ::5] = -1e4
+    z[3] = -INF
+    tokens = torch.zeros(4, dtype=torch.int64, device="cuda")
+    tau, factor = 2.0 ** exponent, 2.0 ** 40
+
+    def grad(logits, temperature, scale):
+        leaf = logits.clone().requires_grad_(True)
+        r = ltc_cuda.ltc_token_logprobs(leaf, tokens, temperature=temperature)
+        w = torch.full((4,), scale, device="cuda")
+        return torch.autograd.grad([r.logprobs, r.entropy], [leaf], [w, w])[0]
+
+    want = grad(z, 1.0, 1.0)
+    assert torch.isfinite(want).all() and bool((want[0, ::3] == 0).all()) and bool((want[0, 1::3] != 0).any())
+    got = grad(z * tau, tau, factor)
+    expected = (want.double() * factor / tau).float()
+    # what the plain call holds below 2^-80 may have been rounded as a subnormal number
+    sure = (want.abs() > 2.0 ** -80) | (want == 0)
+    finite = torch.isfinite(expected) & sure
+    assert torch.equal(got[finite], expected[finite])
+    assert not got[~z.isneginf()].isnan().any() and bool((got[z.isneginf()] == 0).all())
