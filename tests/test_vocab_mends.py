@@ -50,11 +50,13 @@ def test_entropy_gradient_of_masked_rows_under_large_factors(V, exponent):
         return torch.autograd.grad([r.logprobs, r.entropy], [leaf], [w, w])[0]
 
     want = grad(z, 1.0, 1.0)
-    assert torch.isfinite(want).all() and bool((want[0, ::3] == 0).all()) and bool((want[0, 1::3] != 0).any())
+    # the gradient at the token is its own weight less q's share, at a masked token too
+    masked = z.isneginf() & (torch.arange(V, device="cuda") > 0)
+    assert torch.isfinite(want).all() and bool((want[masked] == 0).all()) and bool((want[0, 1::3] != 0).any())
     got = grad(z * tau, tau, factor)
     expected = (want.double() * factor / tau).float()
     # what the plain call holds below 2^-80 may have been rounded as a subnormal number
     sure = (want.abs() > 2.0 ** -80) | (want == 0)
     finite = torch.isfinite(expected) & sure
     assert torch.equal(got[finite], expected[finite])
-    assert not got[~z.isneginf()].isnan().any() and bool((got[z.isneginf()] == 0).all())
+    assert not got.isnan().any() and bool((got[masked] == 0).all())
