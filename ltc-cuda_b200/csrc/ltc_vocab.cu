@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
         for (int w = 0; w < NW; ++w) loss += warp_loss[w];
     }
     if (tid == 0) {
-      g.loss[row] = loss * (g.tau * g.tau * kLn2);
+      g.loss[row] = loss * kLn2 * g.tau * g.tau;  // one factor after the other: tau^2 alone may leave the range
       if (g.stats)
         reinterpret_cast<float4*>(g.stats)[row] = make_float4(t.m, l2, bad ? quiet_nan() : any ? 1.f : 0.f, 0.f);
     }

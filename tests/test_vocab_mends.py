@@ -60,3 +60,23 @@ def test_entropy_gradient_of_masked_rows_under_large_factors(V, exponent):
     finite = torch.isfinite(expected) & sure
     assert torch.equal(got[finite], expected[finite])
     assert not got.isnan().any() and bool((got[masked] == 0).all())
+
+
+@pytest.mark.parametrize("exponent,near", [(-60, False), (-80, False), (40, True), (70, True)])
+def test_distillation_at_extreme_temperatures(exponent, near):
+    """tau^2 by itself is 0 or infinite there, the loss is not.  Powers of two: the loss is that of
+    temperature 1 times tau^2, bit by bit, and a row without entries costs 0."""
+    g = torch.Generator().manual_seed(1)
+    z = torch.randn(5, 2, generator=g).cuda()
+    ids = torch.tensor([[0, 1]] * 4 + [[-1, -1]], device="cuda")
+    if near:  # a loss of about 2^-19 .. 2^-15
+        teacher = z + torch.tensor([0.0, 2.0 ** -6], device="cuda")
+    else:     # a loss of about 2^40
+        z[:, 1] -= 2.0 ** 40
+        teacher = torch.tensor([-(2.0 ** 40), 0.0], device="cuda").expand(5, 2).contiguous()
+    tau = 2.0 ** exponent
+    plain = ltc_cuda.ltc_distill_loss(z, ids, teacher)
+    assert plain[4] == 0 and bool((plain[:4] > 0).all()) and bool(torch.isfinite(plain).all())
+    expected = (plain.double() * tau * tau).float()
+    assert bool((expected[:4] > 2.0 ** -126).all()) and bool(torch.isfinite(expected).all())
+    assert torch.equal(ltc_cuda.ltc_distill_loss(z * tau, ids, teacher * tau, temperature=tau), expected)
