@@ -644,11 +644,12 @@ __global__ void __launch_bounds__(kThreads) vocab_bwd_kernel(VocabArgs g) {
   long long tok = -1;
   if (DISTILL) {
     const float gl = g.g0 ? g.g0[row * g.g0_stride] : 0.f;
-    alpha = st.z != 0.f ? gl * g.tau * st.z : 0.f;  // st.z: 1, or NaN for an id past the vocabulary
+    alpha = gl != 0.f && st.z != 0.f ? gl * g.tau * st.z : 0.f;  // st.z: 1, or NaN for an id past the vocabulary
     extra = -alpha;
   } else {
     tok = g.tokens[row];
-    const float glp = !g.g0 || tok < 0 ? 0.f : tok < g.V ? g.g0[row * g.g0_stride] : quiet_nan();
+    float glp = !g.g0 || tok < 0 ? 0.f : g.g0[row * g.g0_stride];
+    if (glp != 0.f && tok >= g.V) glp = quiet_nan();
     const float gh = g.g1 ? g.g1[row * g.g1_stride] : 0.f;
     alpha = -(gh != 0.f ? fmaf(gh, st.z, glp) : glp) * g.inv_tau;
     beta = -gh * g.inv_tau * kLn2;

@@ -955,7 +955,8 @@ def ltc_token_logprobs(logits, tokens, top_k: int = 0, temperature: float = 1.0)
     lowest id (``None`` when ``top_k`` is 0); where fewer entries are above ``-inf`` they
     hold -1 and ``-inf``.  A row of nothing but ``-inf`` has log probabilities ``-inf``,
     entropy 0 and gradient 0; NaN or ``+inf`` in a row makes its scores NaN and its alternatives
-    unspecified ids.  Differentiable once in ``logits`` through ``logprobs`` and ``entropy``."""
+    unspecified ids.  Differentiable once in ``logits`` through ``logprobs`` and ``entropy``; a row
+    whose two get zero gradients gets zeros, whatever its logits."""
     z, desc = _logits_operand(logits, float(temperature))
     tok = _id_operand(tokens, "tokens", z.device, z.shape[:-1])
     top_k = int(top_k)

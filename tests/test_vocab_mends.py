@@ -80,3 +80,21 @@ def test_distillation_at_extreme_temperatures(exponent, near):
     expected = (plain.double() * tau * tau).float()
     assert bool((expected[:4] > 2.0 ** -126).all()) and bool(torch.isfinite(expected).all())
     assert torch.equal(ltc_cuda.ltc_distill_loss(z * tau, ids, teacher * tau, temperature=tau), expected)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_zero_gradients_of_rows_with_an_id_past_the_vocabulary(dtype):
+    """A row that a zero weight takes out of the loss gets zeros, also where its id makes its loss NaN."""
+    z = torch.randn(3, 300, generator=torch.Generator().manual_seed(0)).to(dtype).cuda()
+    ids = torch.tensor([[1, 300], [2, 3], [1 << 40, -1]], device="cuda")
+    leaf = z.clone().requires_grad_(True)
+    w = torch.tensor([0.0, 1.0, 2.0], device="cuda")
+    loss = ltc_cuda.ltc_distill_loss(leaf, ids, torch.zeros(3, 2, device="cuda"))
+    (g,) = torch.autograd.grad([loss], [leaf], [w])
+    assert (g[0] == 0).all() and torch.isfinite(g[1]).all() and g[2].isnan().any() and (g[1] != 0).any()
+    r = ltc_cuda.ltc_token_logprobs(leaf, ids[:, 1])
+    assert r.logprobs.isnan().tolist() == [True, False, False]
+    (g,) = torch.autograd.grad([r.logprobs], [leaf], [w])
+    assert (g[0] == 0).all() and (g[1] != 0).any() and (g[2] == 0).all()
+    (g,) = torch.autograd.grad([ltc_cuda.ltc_token_logprobs(leaf, ids[:, 1]).logprobs], [leaf], [w + 1])
+    assert g[0].isnan().any()
