@@ -202,7 +202,7 @@ enum { LTC_DTYPE_F32 = 0, LTC_DTYPE_BF16 = 1, LTC_DTYPE_F16 = 2 };
 /* Linear recurrences, parallel over time (ltc_forward walks its T * ode_unfolds unfolds one
  * after the other).  Per channel, inside one sequence:
  *   linear   h_t = a_t h_{t-1} + b_t
- *   gated    L_t = -scale softplus(decay) sigmoid(rate_t),  a_t = exp(L_t),
+ *   gated    L_t = -scale softplus(decay) sigmoid(rate_t),  a_t = exp(L_t),  scale > 0 and finite,
  *            h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(gate_t) x_t
  * Padded batches: inputs (B,T,H), states (B,H), num_seqs = 0, seq_starts NULL.
  * Packed sequences: B = 1, T = all tokens, num_seqs = S in 1..2^30, states (S,H), and seq_starts

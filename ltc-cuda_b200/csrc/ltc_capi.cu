@@ -6,6 +6,7 @@
 //   backward: pack -> recurrent_bwd -> sensory_bwd -> finish (reductions + transforms)
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -910,6 +911,10 @@ int scan_begin(const LtcScanDims* d, const char* who, ScanCall* c) {
   return 0;
 }
 
+int scan_scale(const char* who, float scale) {
+  return scale > 0.f && std::isfinite(scale) ? 0 : fail("%s: scale must be positive and finite", who);
+}
+
 // the forward needs no workspace
 size_t scan_workspace(const ScanCall& c, bool bwd) { return bwd ? c.part_floats * sizeof(float) : 0; }
 
@@ -945,6 +950,7 @@ int scan_args(const LtcScanDims* d, const ScanCall& c, const char* who, const Lt
 int scan_forward(const LtcScanDims* d, const char* who, int policy, const LtcScanInput* const* in,
                  const float* decay, float scale, const float* h0, const int32_t* starts, void* h, float* h_final,
                  void* saved, void* ws, size_t ws_bytes, ltc_stream_t stream) {
+  if (policy && scan_scale(who, scale)) return 1;
   ScanCall c;
   if (scan_begin(d, who, &c)) return 1;
   ScanArgs a{};
@@ -969,6 +975,7 @@ int scan_backward(const LtcScanDims* d, const char* who, int policy, const LtcSc
                   const float* decay, float scale, const float* h0, const int32_t* starts, const void* saved,
                   const LtcScanInput* dh, const float* dh_final, void* const* grads, float* ddecay, float* dh0,
                   void* ws, size_t ws_bytes, ltc_stream_t stream) {
+  if (policy && scan_scale(who, scale)) return 1;
   ScanCall c;
   if (scan_begin(d, who, &c)) return 1;
   ScanArgs a{};
@@ -1084,6 +1091,7 @@ int ltc_gated_scan_step(const LtcScanDims* dims, const LtcScanInput* x, const Lt
                         float* state_out, ltc_stream_t stream) {
   const char* who = "ltc_gated_scan_step";
   if (!dims) return fail("%s: dims is NULL", who);
+  if (scan_scale(who, scale)) return 1;
   LtcScanDims d = *dims;
   d.T = 1;
   d.num_seqs = 0;

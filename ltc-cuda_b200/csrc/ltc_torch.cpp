@@ -295,8 +295,8 @@ py::object gated_step(py::handle x_, py::handle rate_, py::handle gate_, py::han
     if (!THPVariable_Check(o.ptr())) return py::none();
   const bool given = !out_.is_none();
   if ((given && !THPVariable_Check(out_.ptr())) || !PyFloat_Check(scale_.ptr())) return py::none();
-  const double scale = PyFloat_AS_DOUBLE(scale_.ptr());
-  if (!(scale > 0.0) || std::isinf(scale)) return py::none();
+  const float scale = static_cast<float>(PyFloat_AS_DOUBLE(scale_.ptr()));
+  if (!(scale > 0.f) || std::isinf(scale)) return py::none();
   const Tensor &x = THPVariable_Unpack(x_.ptr()), &rate = THPVariable_Unpack(rate_.ptr()),
                &gate = THPVariable_Unpack(gate_.ptr()), &decay = THPVariable_Unpack(decay_.ptr()),
                &state = THPVariable_Unpack(state_.ptr());
@@ -329,8 +329,8 @@ py::object gated_step(py::handle x_, py::handle rate_, py::handle gate_, py::han
       const c10::cuda::CUDAGuard guard(x.device());
       const LtcScanDims d{static_cast<int32_t>(B), 1, static_cast<int32_t>(H), dtype_of(x), 0};
       const LtcScanInput a = input_of(x), b = input_of(rate), c = input_of(gate);
-      check(lib.ltc_gated_scan_step(&d, &a, &b, &c, ptr(decay), static_cast<float>(scale), ptr(state), h.data_ptr(),
-                                    ptr(out), stream_of(x)), "ltc_gated_scan_step");
+      check(lib.ltc_gated_scan_step(&d, &a, &b, &c, ptr(decay), scale, ptr(state), h.data_ptr(), ptr(out),
+                                    stream_of(x)), "ltc_gated_scan_step");
     }
   }
   return py::make_tuple(h, out);

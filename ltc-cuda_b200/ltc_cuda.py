@@ -787,8 +787,8 @@ def _check_decay(decay, device, H: int, scale: float) -> torch.Tensor:
     decay = _as_f32(decay, device, "decay")
     if decay.shape != (H,):
         raise ValueError(f"decay has shape {tuple(decay.shape)}, expected {(H,)}")
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive and finite (got {scale})")
+    if not 0.0 < ctypes.c_float(float(scale)).value < float("inf"):  # the kernels' type
+        raise ValueError(f"scale must be positive and finite in fp32 (got {scale})")
     return decay
 
 

@@ -44,3 +44,24 @@ def test_time_stride_of_a_single_step_is_not_looked_at(monkeypatch):
     wide = torch.empty(((1 << 28) + 2,), dtype=torch.float16).as_strided((1, 2, 1), (1, (1 << 28) + 1, 1))
     with pytest.raises(ValueError, match="time stride"):
         ltc_cuda._scan_operands(("a", "b"), (wide, wide), None, None)
+
+
+def test_scale_has_to_fit_fp32(monkeypatch):
+    """Positive and finite as a double is not enough: 1e39 is infinite and 1e-50 is 0 to the kernels."""
+    monkeypatch.setattr(ltc_cuda, "_on_cuda", lambda *_: None)
+    for scale in (1e39, 1e-50, 0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            ltc_cuda.ltc_gated_scan(t(1, 2, 3), t(1, 2, 3), t(1, 2, 3), t(3), scale=scale)
+        with pytest.raises(ValueError, match="scale"):
+            ltc_cuda.ltc_gated_scan_step(t(2, 3), t(2, 3), t(2, 3), t(3), t(2, 3), scale=scale)
+    for scale in (8, 8.0, torch.tensor(8.0), 3e38):
+        ltc_cuda._check_decay(t(3), t(3).device, 3, scale)
+    lib = ltc_cuda._lib
+    if lib is None:
+        pytest.skip("library not built")
+    dims = ctypes.byref(ltc_cuda.LtcScanDims(1, 2, 3, 0, 0))
+    for scale in (float("inf"), float("nan"), 0.0, -2.0):
+        for rc in (lib.ltc_gated_scan_step(dims, None, None, None, None, scale, None, None, None, None),
+                   lib.ltc_gated_scan_forward(dims, None, None, None, None, scale, *[None] * 6, 0, None),
+                   lib.ltc_gated_scan_backward(dims, None, None, None, None, scale, *[None] * 11, 0, None)):
+            assert rc != 0 and b"scale" in lib.ltc_last_error()
