@@ -256,7 +256,8 @@ int ltc_gated_scan_backward(const LtcScanDims* dims, const LtcScanInput* x, cons
                             const float* dh_final, void* dx, void* drate, void* dgate, float* ddecay, float* dh0,
                             void* workspace, size_t workspace_bytes, ltc_stream_t stream);
 /* One token for each of B sequences (dims.T and num_seqs are ignored, stride_t too): h (B,H)
- * and state_out (B,H), which may be the state array itself.  state may be NULL (zeros). */
+ * and state_out (B,H), which may be the state array itself and shares memory with no operand otherwise.
+ * state may be NULL (zeros). */
 int ltc_gated_scan_step(const LtcScanDims* dims, const LtcScanInput* x, const LtcScanInput* rate,
                         const LtcScanInput* gate, const float* decay, float scale, const float* state, void* h,
                         float* state_out, ltc_stream_t stream);

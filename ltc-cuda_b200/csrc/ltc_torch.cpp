@@ -286,6 +286,17 @@ bool is_floats(const Tensor& t, const Tensor& like, at::IntArrayRef shape) {
   return t.scalar_type() == at::kFloat && t.device() == like.device() && t.sizes() == shape && t.is_contiguous();
 }
 
+// Whether a thread of the step could write into `out` (contiguous, fp32) what another has yet to read
+// from `t`: they share memory and are not the same array, which a thread reads and writes in one place.
+bool clashes(const Tensor& out, const Tensor& t) {
+  if (out.numel() == 0) return false;
+  const char *a = static_cast<const char*>(out.data_ptr()), *b = static_cast<const char*>(t.data_ptr());
+  if (a == b && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == out.numel()) return false;
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return a < b + (last + 1) * t.element_size() && b < a + out.numel() * out.element_size();
+}
+
 // The one-token step: (h, new state), or None for operands that ltc_cuda.py has to look at (to
 // copy them, or to name what is wrong).  In Python these checks took 4 of a call's 10 us, so they
 // come first here, and only what fails them goes through Python's.
@@ -316,8 +327,8 @@ py::object gated_step(py::handle x_, py::handle rate_, py::handle gate_, py::han
   if (given) {
     out = THPVariable_Unpack(out_.ptr());
     if (!is_floats(out, x, x.sizes()) || wants_grad({out})) return py::none();
-    const intptr_t apart = static_cast<char*>(out.data_ptr()) - static_cast<char*>(state.data_ptr());
-    if (apart != 0 && std::abs(apart) < 4 * state.numel()) return py::none();
+    for (const Tensor* t : {&x, &rate, &gate, &decay, &state})
+      if (clashes(out, *t)) return py::none();
   }
   Tensor h;
   {

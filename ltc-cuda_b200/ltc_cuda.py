@@ -826,12 +826,21 @@ def ltc_gated_scan(x, rate, gate, decay, h0=None, seq_starts=None, scale: float 
     return _require_binding().scan(decay, h0, seq_starts, dims, float(scale), tensors)
 
 
+def _clashes(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether ``t`` shares memory with ``out`` (contiguous, fp32) without being the same array."""
+    a, b = out.data_ptr(), t.data_ptr()
+    if out.numel() == 0 or (a == b and t.dtype == out.dtype and t.is_contiguous() and t.numel() == out.numel()):
+        return False
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return a < b + (last + 1) * t.element_size() and b < a + 4 * out.numel()
+
+
 def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_state=None):
     """One token for each sequence: ``x``, ``rate``, ``gate`` ``(B, H)``, ``state`` fp32
     ``(B, H)`` -> ``(h, new_state)``, what :func:`ltc_gated_scan` gives for ``T = 1``.
     ``out_state`` receives the new state; ``out_state=state`` updates it in place, which autograd
-    notices as it does PyTorch's own in-place operations.  Not differentiable: raises where a
-    gradient would be recorded."""
+    notices as it does PyTorch's own in-place operations; it may share memory with no operand
+    otherwise.  Not differentiable: raises where a gradient would be recorded."""
     if _torch_binding is not None:
         done = _torch_binding.gated_step(x, rate, gate, decay, state, out_state, scale)
         if done is not None:
@@ -851,15 +860,16 @@ def ltc_gated_scan_step(x, rate, gate, decay, state, scale: float = 8.0, out_sta
     s = _as_f32(state, dev, "state")
     if s.shape != first.shape:
         raise ValueError(f"state has shape {tuple(s.shape)}, expected {tuple(first.shape)}")
+    inputs = [_rows(t) for t in (x, rate, gate)]
     if out_state is not None:
         if (not isinstance(out_state, torch.Tensor) or out_state.dtype != torch.float32 or out_state.device != dev
                 or out_state.shape != first.shape or not out_state.is_contiguous()):
             raise ValueError("out_state must be a contiguous fp32 tensor shaped and placed like x")
-        if 0 < abs(out_state.data_ptr() - s.data_ptr()) < 4 * s.numel():
-            raise ValueError("out_state may be state itself but not overlap it otherwise")
+        if any(_clashes(out_state, t) for t in (*inputs, decay, s)):
+            raise ValueError("out_state may be state itself but not overlap it or another operand otherwise")
     if _wants_grad(x, rate, gate, decay, state, out_state):
         raise RuntimeError("ltc_gated_scan_step has no backward pass; use ltc_gated_scan or torch.no_grad()")
-    done = _require_binding().gated_step(_rows(x), _rows(rate), _rows(gate), decay, s, out_state, float(scale))
+    done = _require_binding().gated_step(*inputs, decay, s, out_state, float(scale))
     if done is None:
         raise RuntimeError("ltc_cuda.ltc_gated_scan_step: the binding refused checked operands")
     return done

@@ -165,3 +165,17 @@ def test_many_empty_sequences_are_stepped_over():
     want, wl = run("gated", args, None, torch.tensor([0, 1030, N], dtype=torch.int32, device="cuda"))
     assert torch.equal(h, want) and torch.equal(last[[0, -1]], wl) and bool((last[1:-1] == 0).all())
     assert ltc_cuda.wait_timeouts() == 0
+
+
+def test_step_output_overlapping_an_operand_is_refused():
+    """The checks that the binding makes first agree with the ones behind them."""
+    z, d, pool = torch.zeros(2, 4, device="cuda"), torch.zeros(4, device="cuda"), torch.zeros(64, device="cuda")
+    out = pool[8:16].view(2, 4)
+    for args in ((pool[10:18].view(2, 4), z, z, d, z), (z, z, pool[6:30].view(2, 12)[:, :4], d, z),
+                 (z, z, z, pool[8:12], z), (z, z, z, d, pool[9:17].view(2, 4))):
+        with pytest.raises(ValueError, match="overlap"):
+            ltc_cuda.ltc_gated_scan_step(*args, out_state=out)
+    pool.copy_(torch.randn(64, generator=torch.Generator().manual_seed(0)))
+    x = out.clone()
+    want = ltc_cuda.ltc_gated_scan_step(x, x, x, d, x)[1]
+    assert ltc_cuda.ltc_gated_scan_step(out, out, out, d, out, out_state=out)[1] is out and torch.equal(out, want)

@@ -65,3 +65,24 @@ def test_scale_has_to_fit_fp32(monkeypatch):
                    lib.ltc_gated_scan_forward(dims, None, None, None, None, scale, *[None] * 6, 0, None),
                    lib.ltc_gated_scan_backward(dims, None, None, None, None, scale, *[None] * 11, 0, None)):
             assert rc != 0 and b"scale" in lib.ltc_last_error()
+
+
+def test_step_output_may_not_overlap_an_operand(monkeypatch):
+    """Threads of other rows would read what one has written already.  The same array is no
+    overlap: each element is read and written by one thread."""
+    monkeypatch.setattr(ltc_cuda, "_on_cuda", lambda *_: None)
+    monkeypatch.setattr(ltc_cuda, "_torch_binding", None)
+    z, d, pool = t(2, 4), t(4), t(64)
+    out = pool[8:16].view(2, 4)
+    for args in ((pool[10:18].view(2, 4), z, z, d, z), (z, pool[4:12].view(2, 4), z, d, z),
+                 (z, z, pool[6:30].view(2, 12)[:, :4], d, z), (z, z, z, pool[8:12], z), (z, z, z, pool[13:17], z),
+                 (z, z, z, d, pool[9:17].view(2, 4))):
+        with pytest.raises(ValueError, match="overlap"):
+            ltc_cuda.ltc_gated_scan_step(*args, out_state=out)
+    joint = t(3, 24)
+    for args, to in (((out, z, z, d, z), out), ((z, z, z, d, out), out), ((z, out, out, d, out), out),
+                     ((z, z, z, pool[:4], pool[16:24].view(2, 4)), out),
+                     ((*joint[:2, :12].split(4, dim=1), d, z), joint.view(-1)[48:56].view(2, 4)),
+                     ((out.t().contiguous().t(), z, z, d, z), out)):
+        with pytest.raises(RuntimeError):  # taken, as far as the kernels
+            ltc_cuda.ltc_gated_scan_step(*args, out_state=to)
