@@ -15,8 +15,6 @@ from typing import Iterable, List, Optional, Tuple
 import torch
 import torch.distributed as dist
 
-import ltc_cuda
-
 
 def shard_range(total: int, rank: int, world: int) -> Tuple[int, int]:
     """Contiguous [lo, hi) slice of `total` samples for `rank` (sizes differ by at most 1)."""
@@ -71,7 +69,11 @@ def training_step(model, x: torch.Tensor, bucket: FlatGradBucket, optimizer, gro
     whole batch's."""
     bucket.zero()
     out, _ = model(x)
-    loss = out.sum() if teacher is None else ltc_cuda.ltc_distill_loss(out, *teacher, temperature=temperature).sum()
+    if teacher is None:
+        loss = out.sum()
+    else:
+        import ltc_cuda  # only the vocabulary needs the library
+        loss = ltc_cuda.ltc_distill_loss(out, *teacher, temperature=temperature).sum()
     loss.backward()
     bucket.all_reduce(group)
     optimizer.step()
@@ -84,6 +86,7 @@ def evaluation_step(model, x: torch.Tensor, tokens: torch.Tensor, group=None,
     """fp64 ``(sum of log probabilities, sum of entropies, count)`` over the given tokens
     (``(B, T)``, negative: padding) of all ranks' shards, the model's outputs taken as
     logits (``ltc_cuda.ltc_token_logprobs``)."""
+    import ltc_cuda
     out, _ = model(x)
     scores = ltc_cuda.ltc_token_logprobs(out, tokens, temperature=temperature)
     given = tokens >= 0
