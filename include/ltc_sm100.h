@@ -225,7 +225,8 @@ typedef struct {
   int64_t stride_b, stride_t;
 } LtcScanInput;
 
-/* saved_bytes: state before every 32nd token, kept by a forward for its backward (0 up to
+/* The forward needs no workspace: fwd_workspace_bytes is 0, and its workspace may be NULL.
+ * saved_bytes: state before every 32nd token, kept by a forward for its backward (0 up to
  * 32 tokens).  cluster: blocks that share one sequence x 32 channels where there are too few
  * of those to fill the GPU. */
 typedef struct {

@@ -275,7 +275,6 @@ struct VocabArgs {
   void* dz;                  // (rows, V)
   // set per launch
   int cluster, chunk, chunks;
-  long long blocks;          // rows at work at a time (forward)
 };
 cudaError_t launch_vocab_fwd(VocabArgs a, int dtype, bool distill, int num_sms, cudaStream_t st);
 cudaError_t launch_vocab_bwd(VocabArgs a, int dtype, bool distill, cudaStream_t st);
