@@ -363,11 +363,15 @@ __device__ __forceinline__ void exchange_end(int cl) {
 
 // The warps' folds are in shared memory: makes them visible to the block and sends the block's
 // fold (in time order) to all blocks of the cluster, each warp to its share of them.  The
-// messages complete bytes on the receiver's barrier, so that no block waits for its own.
+// messages complete bytes on the receiver's barrier, so that no block waits for its own.  The slot of
+// the round before is armed for the round behind here, away from the waits: its messages may come
+// first, since the phase stays open for this arrival.
 template <bool PACKED, bool REVERSE, int NW, int NF, bool MANY>
-__device__ __forceinline__ void exchange_send(Exchange<NW, NF, MANY>& sh, int buf, int cl, int rank) {
+__device__ __forceinline__ void exchange_send(Exchange<NW, NF, MANY>& sh, int buf, int cl, int rank, bool first) {
+  const int expired = MANY && cl > 1 ? *static_cast<volatile int*>(&sh.aborted) : 0;
   __syncthreads();
-  if (!MANY || cl == 1 || *static_cast<volatile int*>(&sh.aborted)) return;
+  if (!MANY || cl == 1 || expired) return;
+  if (threadIdx.x == 0 && !first) mbar_arm(smem_addr(&sh.bar[buf ^ 1]), message_bytes(cl));
   const int ch = threadIdx.x & 31;  // a narrow item's upper half sends what nobody reads
   float A = 1.f, B = 0.f;
   int F = 0;
@@ -397,7 +401,6 @@ __device__ __forceinline__ void exchange_wait(Exchange<NW, NF, MANY>& sh, int bu
   if (!MANY || cl == 1) return;
   const unsigned bar = smem_addr(&sh.bar[buf]);
   mbar_wait(bar, phase, &sh.aborted, &g_scan_wait_timeouts);
-  if (threadIdx.x == 0 && !*static_cast<volatile int*>(&sh.aborted)) mbar_arm(bar, message_bytes(cl));
 }
 
 // (A, B) of this thread's channels
@@ -639,7 +642,7 @@ __global__ void __launch_bounds__(S::THREADS, (fwd_blocks<P, T, S, MANY>())) sca
         store(&sh.w[buf][wt][1][lx * VEC], B);
         if (PACKED && lx == 0) sh.wf[buf][wt] = F;
       }
-      exchange_send<PACKED, false>(sh, buf, cl, it.rank);
+      exchange_send<PACKED, false>(sh, buf, cl, it.rank, round == 0);
       if (PACKED && round + 1 < g.rounds) {  // while the messages are on their way
         next = walk.template marks<R, S::TT>(t0 + cl * S::TT - ty * R, t0 + cl * S::TT);
         if (next.first && g.h0) hz = load_f32<V>(g.h0 + (long long)next.nf * g.H + cr);
@@ -879,7 +882,7 @@ __global__ void __launch_bounds__(S::THREADS, (bwd_blocks<P, T, S, MANY>())) sca
         store(&sh.w[buf][wt][2][lx * VEC], Ct);
         if (PACKED && lx == 0) sh.wf[buf][wt] = F | Fo;
       }
-      exchange_send<PACKED, true>(sh, buf, cl, it.rank);
+      exchange_send<PACKED, true>(sh, buf, cl, it.rank, round == g.rounds - 1);
       if (PACKED && round > 0) {
         next = walk.template marks<R, S::TT>(t0 - cl * S::TT - ty * R, t0 - cl * S::TT);
         if (next.first && g.h0) hz = load_f32<V>(g.h0 + (long long)next.nf * g.H + cr);
