@@ -1,11 +1,11 @@
 // Torch binding of the sequence operators: output allocation, autograd and the calls into
 // libltc_sm100.so without Python on the way.
 //
-// Measured: through ctypes and a Python autograd.Function a one-token step of 24 x 64 took 16.6 us
-// a call and a training pass whose kernels take 55 us took 109 (the backward, on autograd's device
-// thread, waits for the interpreter); here 6.2 and 71 us.  Argument checks stay in ltc_cuda.py, but
-// for the step's.  The library is not linked: ltc_cuda.py passes the addresses of its entry points,
-// so that LTC_SM100_LIB selects the library here too.
+// Measured: through ctypes and a Python autograd.Function a pass with a one-token step of 24 x 64 took
+// 16.6 us and a training pass whose kernels take 55 us took 109 (the backward, on autograd's device
+// thread, waits for the interpreter); here 8.4 and 74 us (the step by itself 5.9).  Argument checks stay
+// in ltc_cuda.py, but for the step's.  The library is not linked: ltc_cuda.py passes the addresses of
+// its entry points, so that LTC_SM100_LIB selects the library here too.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -298,7 +298,7 @@ bool clashes(const Tensor& out, const Tensor& t) {
 }
 
 // The one-token step: (h, new state), or None for operands that ltc_cuda.py has to look at (to
-// copy them, or to name what is wrong).  In Python these checks took 4 of a call's 10 us, so they
+// copy them, or to name what is wrong).  In Python these checks took 4 us of a call, so they
 // come first here, and only what fails them goes through Python's.
 py::object gated_step(py::handle x_, py::handle rate_, py::handle gate_, py::handle decay_, py::handle state_,
                       py::handle out_, py::handle scale_) {
