@@ -575,7 +575,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
     float loss = 0.f;
     bool bad = false;
     if (busy) {
-      const float le = log2f(es);
+      // tau (log p - log q) in the logits' own units: a masked entry at the type's lowest value stays
+      // finite as long as the loss does.  The other tau comes before the sum where it is small and
+      // after it where it is large, so that no term leaves the range before the sum does.
+      const float le = log2f(es), tl = g.tau * kLn2;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         float pk = 0.f;
@@ -583,7 +586,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
         if (id[e] >= 0 && any) {
           pk = te[e] / es;
           if (pk != 0.f && id[e] < g.V)
-            loss = fmaf(pk, (t_id[e] - em) * c2 - le - (empty ? neg_inf() : (z_id[e] - t.m) * c2 - l2), loss);
+            loss = fmaf(pk * fminf(g.tau, 1.f),
+                        empty ? -neg_inf() : fmaf(tl, l2 - le, (t_id[e] - em) - (z_id[e] - t.m)), loss);
         }
         if (e * NT + tid < entries && g.probs) g.probs[row * g.K + e * NT + tid] = pk;
       }
@@ -600,7 +604,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) vocab_fwd_kernel(VocabArgs g) {
         for (int w = 0; w < NW; ++w) loss += warp_loss[w];
     }
     if (tid == 0) {
-      g.loss[row] = loss * kLn2 * g.tau * g.tau;  // one factor after the other: tau^2 alone may leave the range
+      g.loss[row] = loss * fmaxf(g.tau, 1.f);
       if (g.stats)
         reinterpret_cast<float4*>(g.stats)[row] = make_float4(t.m, l2, bad ? quiet_nan() : any ? 1.f : 0.f, 0.f);
     }

@@ -98,3 +98,26 @@ def test_zero_gradients_of_rows_with_an_id_past_the_vocabulary(dtype):
     assert (g[0] == 0).all() and (g[1] != 0).any() and (g[2] == 0).all()
     (g,) = torch.autograd.grad([ltc_cuda.ltc_token_logprobs(leaf, ids[:, 1]).logprobs], [leaf], [w + 1])
     assert g[0].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("tau", [0.25, 1.0, 2.0])
+def test_distillation_of_entries_masked_by_the_lowest_value(dtype, tau):
+    """A teacher's entry that the student masks with the type's lowest value costs p |lowest| tau:
+    a loss within fp32's range, where |lowest| / (tau ln 2) is not."""
+    g = torch.Generator().manual_seed(3)
+    z = torch.randn(6, 700, generator=g).to(dtype).cuda()
+    ids = torch.randint(0, 700, (6, 5), generator=g).cuda()
+    teacher = torch.randn(6, 5, generator=g).cuda() * 2
+    teacher[:, 0] -= 8
+    low = torch.finfo(dtype).min
+    z[torch.arange(6, device="cuda"), ids[:, 0]] = low
+    loss = ltc_cuda.ltc_distill_loss(z, ids, teacher, temperature=tau)
+    w, t = z.cpu().double() / tau, teacher.cpu().double() / tau
+    p = torch.softmax(t, 1)
+    want = tau * tau * (p * (torch.log_softmax(t, 1) - torch.log_softmax(w, 1).gather(1, ids.cpu()))).sum(1)
+    assert bool((want < 3e38).all()) and bool((want > 1e12).all())  # all but nothing is the masked entry's
+    # p of that entry is off by 4 U times its distance from the largest and 25 U more (two exponentials, the sum
+    # of five, a division); the products and the sum round ten times
+    off = (4 * (t.max(1).values - t[:, 0]) + 35) * 2.0 ** -24
+    assert bool(((loss.cpu().double() - want).abs() <= off * want).all())
