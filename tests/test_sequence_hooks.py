@@ -121,3 +121,24 @@ def test_another_type_or_shape_is_refused():
         for o, leaf in zip(outs, (z, z, x, x)):
             with pytest.raises(RuntimeError, match="came back"):
                 torch.autograd.grad(o.sum(), leaf)
+
+
+def test_recomputed_in_the_backward():
+    """Scan, head and both losses inside a checkpoint: saved tensors are the recomputation's."""
+    from torch.utils.checkpoint import checkpoint
+    base, head, decay = normal(B, 70, 3 * H, seed=7), normal(H, V, seed=8), normal(H, seed=9) - 3
+    ids = torch.randint(0, V, (B, 69, 3), generator=torch.Generator().manual_seed(2)).cuda()
+    teacher = normal(B, 69, 3, seed=10)
+
+    def loss(x, w, d):
+        h, last = ltc_cuda.ltc_gated_scan(*x.split(H, dim=-1), d)
+        z = (h @ w)[:, :-1]
+        r = ltc_cuda.ltc_token_logprobs(z, ids[..., 0])
+        return ltc_cuda.ltc_distill_loss(z, ids, teacher).sum() + r.entropy.sum() + last.square().sum()
+
+    def grads(run):
+        leaves = [t.clone().requires_grad_(True) for t in (base, head, decay)]
+        return torch.autograd.grad(run(*leaves), leaves)
+
+    for g, w in zip(grads(lambda *a: checkpoint(loss, *a, use_reentrant=False)), grads(loss)):
+        assert torch.equal(g, w)
